@@ -1,0 +1,97 @@
+// Launcher of the attention over the 8-bit cache (attention_q8.cuh).
+#include "attention_q8.cuh"
+
+namespace cbis {
+extern template int q8_run<32>(const Q8Args&, const Q8Plan&, bool, int, cudaStream_t);
+extern template int q8_run<64>(const Q8Args&, const Q8Plan&, bool, int, cudaStream_t);
+extern template int q8_run<128>(const Q8Args&, const Q8Plan&, bool, int, cudaStream_t);
+extern template int q8_run<256>(const Q8Args&, const Q8Plan&, bool, int, cudaStream_t);
+}  // namespace cbis
+
+using namespace cbis;
+
+namespace {
+
+int padded_width(int hd) { return hd <= 32 ? 32 : (hd <= 64 ? 64 : (hd <= 128 ? 128 : 256)); }
+
+// Columns of queries / 8: as many as the query heads and rows that share keys fill, up to what the accumulators' registers allow.
+int columns8(int hdp, int f32, long long queries) {
+  const int most = hdp == 256 ? (f32 ? 1 : 2) : (f32 ? 2 : 4);
+  const int nt = queries <= 8 ? 1 : (queries <= 16 ? 2 : 4);
+  return nt < most ? nt : most;
+}
+int blocks_per_sm(int hdp, int nt, int f32) { return hdp == 256 ? 2 : (nt == 1 && !f32 ? 4 : (nt == 4 || f32 ? 2 : 3)); }
+
+// rows_of_seg 0: decoding, `n` rows; else `n` requests of at most so many rows.
+Q8Plan q8_plan(int n, int rows_of_seg, int n_head, int n_kv_head, int hd, int f32, int max_context) {
+  Q8Plan p = {};
+  const int group = n_head / n_kv_head;
+  p.hdp = padded_width(hd);
+  p.nt = columns8(p.hdp, f32, (long long)group * (rows_of_seg ? rows_of_seg : 1));
+  p.heads_per = group < 8 * p.nt ? group : 8 * p.nt;
+  p.head_blocks = (group + p.heads_per - 1) / p.heads_per;
+  p.rows_per = rows_of_seg ? 8 * p.nt / p.heads_per : 1;
+  p.tiles_per_seg = rows_of_seg ? (rows_of_seg + p.rows_per - 1) / p.rows_per : 1;
+  p.items = (long long)n * p.tiles_per_seg;
+  const long long unit = p.hdp <= 64 ? 128 : 64, pairs = p.items * n_kv_head * p.head_blocks;
+  const long long units = pairs * ((max_context + unit - 1) / unit + 1), slots = 148LL * blocks_per_sm(p.hdp, p.nt, f32);
+  p.blocks = units < slots ? units : slots;
+  p.floats = p.blocks * 2 * 8 * p.nt * (p.hdp + 2);
+  p.counters = pairs;
+  return p;
+}
+
+}  // namespace
+
+// Scratch of a launch over `n` decoding rows (rows_of_seg 0) or `n` requests of at most rows_of_seg rows: floats for partial results
+// and counters (zero before the first launch; every launch leaves them zero).  Returns a status.
+CBIS_EXPORT int cbis_attention_q8_scratch(int n, int rows_of_seg, int n_head, int n_kv_head, int hd, int dtype, int max_context,
+                                          long long* floats, long long* counters) {
+  *floats = *counters = 0;
+  if (n <= 0) return CBIS_OK;
+  if (n_kv_head <= 0 || n_head <= 0 || n_head % n_kv_head || hd <= 0 || hd > 256 || rows_of_seg < 0 || max_context < 0) return CBIS_ERR_BAD_SIZE;
+  const Q8Plan p = q8_plan(n, rows_of_seg, n_head, n_kv_head, hd, dtype == CBIS_F32, max_context);
+  *floats = p.floats;
+  *counters = p.counters;
+  return p.items > Q8_MAX_ITEMS ? CBIS_ERR_TOO_LARGE : CBIS_OK;
+}
+
+// rows_of_seg 0: n decoding rows (row_seq, positions; with k_off >= 0 the current token's key and value are taken from q's rows, quantised
+// and stored at slot_mapping[row]); else the n requests from seg0 on, whose rows are cu_rows[s] .. cu_rows[s + 1] - 1 at positions from
+// seg_start[s] on.  A row whose request is no row of the block table, or that sees no key, gets zeros.
+CBIS_EXPORT int cbis_attention_q8(const void* q, int ld, int k_off, int v_off, void* kc, void* ks, void* vc, void* vs, const int* block_table,
+                                  int max_blocks, int n_seqs, int num_pages, const int* row_seq, const int* positions,
+                                  const int* slot_mapping, const int* cu_rows, const int* seg_start, int seg0, int n, int rows_of_seg, int n_rows,
+                                  void* out, int out_ld, float* part, long long part_floats, unsigned* counters, long long n_counters,
+                                  int n_head, int n_kv_head, int hd, int ps, float scale, int window, int max_context, int dtype,
+                                  void* stream, const float* sinks, const float* slopes, const float* rates, float temp_coef,
+                                  int temp_every, float cap, int keep) {
+  if (n <= 0) return CBIS_OK;
+  if (dtype != CBIS_F32 && dtype != CBIS_BF16) return CBIS_ERR_BAD_DTYPE;
+  if (hd <= 0 || hd > 256 || hd % 16 || ps <= 0 || n_kv_head <= 0 || n_head <= 0 || n_head % n_kv_head || max_blocks <= 0 || keep < 0 ||
+      num_pages < 0 || rows_of_seg < 0 || max_context < 0 || n_rows < 0 || (rows_of_seg && (seg0 < 0 || seg0 + n > n_seqs)) || (!rows_of_seg && n > n_rows))
+    return CBIS_ERR_BAD_SIZE;
+  if ((long long)max_blocks * ps > 0x7fffff00LL || (long long)num_pages * ps > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
+  const int f32 = dtype == CBIS_F32, align = f32 ? 4 : 8;
+  if (ld % align || (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15)) return CBIS_ERR_ALIGNMENT;
+  const Q8Plan p = q8_plan(n, rows_of_seg, n_head, n_kv_head, hd, f32, max_context);
+  if (p.items > Q8_MAX_ITEMS) return CBIS_ERR_TOO_LARGE;
+  if (part_floats < p.floats || n_counters < p.counters || (k_off >= 0 && slot_mapping == nullptr)) return CBIS_ERR_BAD_SIZE;
+  Q8Args a = {};
+  a.q = q; a.out = out; a.kc = (int8_t*)kc; a.vc = (int8_t*)vc; a.ks = (float*)ks; a.vs = (float*)vs;
+  a.block_table = block_table; a.row_seq = row_seq; a.positions = positions; a.slot_mapping = slot_mapping;
+  a.cu_rows = rows_of_seg ? cu_rows : nullptr; a.seg_start = seg_start; a.part = part; a.counters = counters;
+  a.sinks = sinks; a.slopes = slopes; a.rates = rates;
+  a.n_rows = n_rows; a.ld = ld; a.out_ld = out_ld; a.k_off = k_off; a.v_off = v_off; a.max_blocks = max_blocks; a.num_pages = num_pages; a.n_seqs = n_seqs;
+  a.seg0 = seg0; a.n_items = (int)p.items; a.tiles_per_seg = p.tiles_per_seg; a.n_head = n_head; a.n_kv_head = n_kv_head;
+  a.heads_per = p.heads_per; a.head_blocks = p.head_blocks; a.rows_per = p.rows_per;
+  a.hd = hd; a.ps = ps; a.window = window; a.keep = keep; a.temp_every = temp_every; a.scale = scale; a.cap = cap; a.temp_coef = temp_coef;
+  const bool ext = cap > 0.f || (keep > 0 && window != 0) || slopes || temp_every > 0;
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (p.hdp) {
+    case 32: return q8_run<32>(a, p, ext, f32, st);
+    case 64: return q8_run<64>(a, p, ext, f32, st);
+    case 128: return q8_run<128>(a, p, ext, f32, st);
+    default: return q8_run<256>(a, p, ext, f32, st);
+  }
+}

@@ -1,0 +1,6 @@
+// Attention over the 8-bit cache (attention_q8.cuh) for widths padded to 32.
+#include "attention_q8.cuh"
+
+namespace cbis {
+template int q8_run<32>(const Q8Args&, const Q8Plan&, bool, int, cudaStream_t);
+}

@@ -1,0 +1,31 @@
+// The 8-bit form of a cached row (one token's key or value of one head): a 32-bit scale and a signed 8-bit code per number,
+//     scale = max(amax / 127, 2^-120),   code = the whole number nearest to x / scale, ties to even,   value = code * scale.
+// The code is the one nearest by the exact quotient, not by a rounded one: half steps are common (x = amax / 2 is one, and 16-bit
+// rows hold it often), and there a rounded quotient gives one code or the other by chance.  A row with an infinity or a NaN has
+// scale NaN and codes 0: every value read back from it is NaN.  The floor of the scale keeps its reciprocal finite; numbers below
+// 2^-121 are read back as 0.
+#pragma once
+#include "common.cuh"
+
+namespace cbis {
+
+constexpr float Q8_FLOOR = 7.52316384526264e-37f;      // 2^-120
+
+// The largest magnitude as the bits of |x|: ordered like the magnitudes, an infinity above every number and a NaN above that.
+__device__ __forceinline__ unsigned q8_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+__device__ __forceinline__ float q8_scale(unsigned amax_bits) {
+  return amax_bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__fdiv_rn(__uint_as_float(amax_bits), 127.f), Q8_FLOOR);
+}
+
+// inv: the reciprocal of the scale.  q is at most one step off; the remainder x - q scale is exact in 32 bits.
+__device__ __forceinline__ int q8_code(float x, float scale, float inv) {
+  float q = rintf(x * inv);
+  const float r = fmaf(-q, scale, x), half = 0.5f * scale;
+  const bool odd = ((int)q & 1) != 0;
+  if (r > half || (r == half && odd)) q += 1.f;
+  if (r < -half || (r == -half && odd)) q -= 1.f;
+  return scale == scale ? (int)q : 0;
+}
+
+}  // namespace cbis

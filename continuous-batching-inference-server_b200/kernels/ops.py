@@ -10,7 +10,7 @@ from __future__ import annotations
 import ctypes
 import weakref
 from ctypes import c_float, c_int, c_void_p
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -539,6 +539,305 @@ def kv_write(qkv, k_off, v_off, k_cache, v_cache, slot_mapping, n_kv_head, head_
                                  _ptr(v_cache), _ptr(slot_mapping), c_int(T), c_int(n_kv_head), c_int(head_dim),
                                  c_int(page_size), c_int(dtype_code(qkv.dtype)), _stream(), c_int(v_head_dim))
     _check(st, "kv_write", f"T={T} kv_heads={n_kv_head} head_dim={head_dim} page={page_size}")
+
+
+# ---- the 8-bit cache -------------------------------------------------------------------------------------------------
+class Q8Pages(NamedTuple):
+    """One cached array in 8 bits: ``codes`` int8 ``[pages, heads, page_size, width]``, ``scales`` float32 ``[pages, heads, page_size]``.
+    A token's row of one head stands for code * scale, with scale = max(amax / 127, 2^-120) of the row that was written and each code
+    the whole number nearest to x / scale (ties to even).  A row with an infinity or a NaN has scale NaN: all of it reads back as NaN."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def q8_pages(num_pages: int, heads: int, page_size: int, width: int, device="cuda") -> Q8Pages:
+    """Pages of zeros."""
+    return Q8Pages(torch.zeros((num_pages, heads, page_size, width), dtype=torch.int8, device=device),
+                   torch.zeros((num_pages, heads, page_size), dtype=torch.float32, device=device))
+
+
+_q8_fns = {}
+
+
+def _q8_fn(name: str, argtypes):
+    fn = _q8_fns.get(name)
+    if fn is None:
+        fn = getattr(kernels(), name)
+        fn.argtypes = argtypes
+        _q8_fns[name] = fn
+    return fn
+
+
+_P, _I, _F, _L = c_void_p, c_int, c_float, ctypes.c_longlong
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _q8_need(ok, what: str, why: str) -> None:
+    if not ok:
+        raise KernelError(f"{what}: {why}")
+
+
+def _q8_here(what: str, *ts) -> None:
+    """All tensors on the current CUDA device, whose current stream takes the launch."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise KernelError(f"{what}: kernels take CUDA tensors only; there is no CPU path")
+        if dev is None:
+            dev = t.device
+            here = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+            if dev.index != here:
+                raise KernelError(f"{what}: the tensors are on {dev}, the current device is cuda:{here}")
+        elif t.device != dev:
+            raise KernelError(f"{what}: tensors on {dev} and {t.device}")
+
+
+def _q8_array(what: str, name: str, pages: Q8Pages, heads: int, page_size: int, width: int) -> None:
+    c, s = pages
+    _q8_need(c.dtype == torch.int8 and s.dtype == torch.float32, what, f"the {name} need int8 codes and float32 scales")
+    _q8_need(c.dim() == 4 and c.shape[1:] == (heads, page_size, width) and c.is_contiguous(), what,
+             f"the {name}' codes are not contiguous [pages, {heads}, {page_size}, {width}]")
+    _q8_need(s.shape == c.shape[:3] and s.is_contiguous(), what, f"the {name}' scales are not contiguous {tuple(c.shape[:3])}")
+
+
+def _q8_int32(what: str, name: str, t, numel: int) -> None:
+    _q8_need(t is not None and t.dtype == torch.int32 and t.is_contiguous() and t.numel() >= numel, what,
+             f"{name} must be contiguous int32 with at least {numel} entries")
+
+
+def _q8_table(what: str, block_table) -> None:
+    _q8_need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.is_contiguous() and block_table.shape[1] > 0, what,
+             "the block table must be contiguous int32 [requests, blocks]")
+
+
+def kv_write_q8(qkv, k_off, v_off, k_pages, v_pages, slot_mapping, n_kv_head, head_dim, page_size, v_head_dim=0):
+    """``kv_write`` into an 8-bit cache: rows of this step's K and V (columns k_off.. and v_off.. of qkv, bfloat16 or float32) are
+    quantised, a scale per token and head, and go to their token slots (a slot that the cache does not have writes nothing).
+    ``v_head_dim``: the values' width where it is not the keys'.  ``v_pages`` None, or the keys' own pages: one array stands for
+    both and takes the rows at k_off."""
+    what = "kv_write_q8"
+    vd = int(v_head_dim) or head_dim
+    if v_pages is not None and v_pages.codes is k_pages.codes:
+        v_pages = None
+    T = qkv.shape[0]
+    code = dtype_code(qkv.dtype)
+    _q8_need(qkv.dim() == 2 and (T == 0 or qkv.stride(1) == 1) and k_off >= 0 and k_off + n_kv_head * head_dim <= qkv.shape[1]
+             and (v_pages is None or (v_off >= 0 and v_off + n_kv_head * vd <= qkv.shape[1])), what,
+             f"{n_kv_head} heads of {head_dim} and {vd} at columns {k_off} and {v_off} do not lie in rows of {tuple(qkv.shape)}")
+    _q8_array(what, "keys", k_pages, n_kv_head, page_size, head_dim)
+    if v_pages is not None:
+        _q8_array(what, "values", v_pages, n_kv_head, page_size, vd)
+        _q8_need(v_pages.codes.shape[0] == k_pages.codes.shape[0], what, "keys and values have different numbers of pages")
+    _q8_int32(what, "slot_mapping", slot_mapping, T)
+    vc, vs = (None, None) if v_pages is None else v_pages
+    _q8_here(what, qkv, k_pages.codes, k_pages.scales, vc, vs, slot_mapping)
+    if T == 0:
+        return
+    fn = _q8_fn("cbis_kv_write_q8", [_P, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P])
+    st = fn(_at(qkv), qkv.stride(0), k_off, v_off, _at(k_pages.codes), _at(k_pages.scales), _at(vc), _at(vs), _at(slot_mapping),
+            k_pages.codes.shape[0] * page_size, T, n_kv_head, head_dim, vd, page_size, code, _stream())
+    _check(st, what, f"T={T} kv_heads={n_kv_head} head_dim={head_dim} page={page_size}")
+
+
+def kv_read_q8(k_pages, v_pages, k_out, v_out, block_table, seg_start, seg_ctx, max_tokens, window=0, keep=0, whole_pages=False):
+    """Values of an 8-bit cache in bfloat16 or float32: what stands in page p of ``k_pages`` and ``v_pages`` goes to page p of ``k_out`` and
+    ``v_out`` ``[pages, heads, page_size, width]``, for the tokens that the queries of request s (a row of ``block_table``) at
+    positions ``seg_start[s]`` .. ``seg_ctx[s]`` - 1 see under ``window`` and ``keep`` (as in ``paged_attention_generic``); everything else in
+    the two stays as it is.  ``max_tokens``: no request has more than so many such tokens, the kept first ones aside.
+    ``whole_pages``: what the request holds beside them in their pages is read back too; any kernel that takes pages then reads ``k_out`` and
+    ``v_out`` through the same block table.  ``v_pages`` None: one array."""
+    what = "kv_read_q8"
+    if v_pages is not None and v_pages.codes is k_pages.codes:
+        v_pages = v_out = None
+    _q8_need(k_pages.codes.dim() == 4, what, "the keys' codes are not [pages, heads, page_size, width]")
+    P, G, ps, hd = k_pages.codes.shape
+    _q8_array(what, "keys", k_pages, G, ps, hd)
+    _q8_table(what, block_table)
+    S = block_table.shape[0]
+    code = dtype_code(k_out.dtype)
+    outs = [(k_out, k_pages)]
+    vd = hd
+    if v_pages is not None:
+        vd = v_pages.codes.shape[-1]
+        _q8_array(what, "values", v_pages, G, ps, vd)
+        outs.append((v_out, v_pages))
+    for o, p in outs:
+        _q8_need(o is not None and o.dtype == k_out.dtype and o.shape == p.codes.shape and p.codes.shape[0] == P and o.is_contiguous(), what,
+                 "the values' pages must be contiguous, of one type and of the codes' shape")
+    _q8_int32(what, "seg_start", seg_start, S)
+    _q8_int32(what, "seg_ctx", seg_ctx, S)
+    _q8_need(keep >= 0, what, "keep is negative")
+    vc, vs = (None, None) if v_pages is None else v_pages
+    _q8_here(what, k_pages.codes, k_pages.scales, vc, vs, k_out, v_out, block_table, seg_start, seg_ctx)
+    if S == 0 or max_tokens <= 0 or P == 0:
+        return
+    fn = _q8_fn("cbis_kv_read_q8", [_P, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P])
+    st = fn(_at(k_pages.codes), _at(k_pages.scales), _at(vc), _at(vs), _at(k_out), _at(v_out) if v_pages is not None else None,
+            _at(block_table), block_table.shape[1], P, _at(seg_start), _at(seg_ctx), S, int(max_tokens), G, hd, vd, ps, int(window),
+            int(keep), int(bool(whole_pages)), code, _stream())
+    _check(st, what, f"requests={S} heads={G} widths={hd}/{vd} page={ps}")
+
+
+ATTENTION_Q8_MAX_HEAD_DIM = 256
+
+
+def attention_q8_takes(head_dim: int, v_head_dim: int = 0) -> bool:
+    """Whether ``paged_decode_q8`` and ``paged_prefill_q8`` take these widths: equal ones, a multiple of 16 up to 256.  For any other the
+    cache is read back (``kv_read_q8``) and attended to as one of 16 or 32 bits."""
+    return (v_head_dim or head_dim) == head_dim and head_dim % 16 == 0 and 16 <= head_dim <= ATTENTION_Q8_MAX_HEAD_DIM
+
+
+def _q8_scratch(n, rows_of_seg, n_head, n_kv_head, head_dim, code, max_context):
+    fn = _q8_fn("cbis_attention_q8_scratch", [_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_L), ctypes.POINTER(_L)])
+    floats, counters = _L(), _L()
+    return fn(n, rows_of_seg, n_head, n_kv_head, head_dim, code, max_context, ctypes.byref(floats), ctypes.byref(counters)), floats.value, counters.value
+
+
+def attention_q8_scratch(rows: int, max_seg_rows: int, n_seg: int, n_head: int, n_kv_head: int, head_dim: int, max_context: int, dtype):
+    """(floats, int32 counters) that ``paged_decode_q8`` over ``rows`` rows and ``paged_prefill_q8`` over ``n_seg`` requests of ``rows``
+    rows in all, at most ``max_seg_rows`` each, need; the counters are zero before the first launch, and every launch leaves them zero."""
+    code = dtype_code(dtype)
+    if max_seg_rows <= 1:
+        st, floats, counters = _q8_scratch(max(rows, n_seg), 0, n_head, n_kv_head, head_dim, code, max_context)
+        _check(st, "attention_q8_scratch", f"rows={rows} heads={n_head}/{n_kv_head} head_dim={head_dim}", 0)
+        return max(floats, 1), max(counters, 1)
+    st, floats, counters = _q8_scratch(n_seg, max_seg_rows, n_head, n_kv_head, head_dim, code, max_context)
+    if st not in (0, -4):      # -4: too many row tiles for the kernel that reads codes; a longer chunk's cache is read back
+        _check(st, "attention_q8_scratch", f"requests={n_seg} heads={n_head}/{n_kv_head} head_dim={head_dim}", 0)
+    n, _ = _prefill_q8_chunks(max_seg_rows, n_seg, n_head, head_dim, max_context, dtype)
+    return max(floats, rows * n_head * n * (head_dim + 4), 1), max(counters, 1)
+
+
+def _prefill_q8_chunks(max_seg_rows, n_seg, n_head, head_dim, max_context, dtype):
+    """The key chunks of the kernel that attends to the values read back."""
+    if dtype == torch.bfloat16 and head_dim in (64, 128) and USE_TCGEN05:
+        return prefill_key_chunks(-(-max_seg_rows // 128), n_head, n_seg, max_context, 2, 2, 8192)
+    return prefill_key_chunks(-(-max_seg_rows // 64), n_head, n_seg, max_context, 1, 8 if dtype == torch.bfloat16 else 16)
+
+
+def _q8_attention_checks(what, q, k_pages, v_pages, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, slopes,
+                         sinks, rates, keep):
+    _q8_need(attention_q8_takes(head_dim), what, f"head_dim={head_dim} is no multiple of 16 up to {ATTENTION_Q8_MAX_HEAD_DIM}")
+    _q8_need(n_kv_head > 0 and n_head > 0 and n_head % n_kv_head == 0, what, f"n_head={n_head} is not a multiple of n_kv_head={n_kv_head}")
+    _q8_array(what, "keys", k_pages, n_kv_head, page_size, head_dim)
+    _q8_array(what, "values", v_pages, n_kv_head, page_size, head_dim)
+    _q8_need(v_pages.codes.shape[0] == k_pages.codes.shape[0], what, "keys and values have different numbers of pages")
+    _q8_table(what, block_table)
+    _q8_need(q.dim() == 2 and q.stride(1) == 1 and q.shape[1] >= n_head * head_dim, what, f"{n_head} heads of {head_dim} do not fit rows of {tuple(q.shape)}")
+    _q8_need(out.dim() == 2 and out.dtype == q.dtype and out.stride(1) == 1 and out.shape[0] >= q.shape[0] and out.shape[1] >= n_head * head_dim,
+             what, "out must have q's type and rows and room for the heads")
+    _q8_need(scratch.dtype == torch.float32 and scratch.is_contiguous(), what, "scratch must be contiguous float32")
+    _q8_need(counters.dtype == torch.int32 and counters.is_contiguous(), what, "counters must be contiguous int32")
+    for name, x in (("slopes", slopes), ("sinks", sinks), ("rates", rates)):
+        _q8_need(x is None or (x.dtype == torch.float32 and x.numel() == n_head and x.is_contiguous()), what, f"{name} must be {n_head} float32 numbers")
+    _q8_need(rates is None or slopes is not None, what, "rates need slopes")
+    _q8_need(keep >= 0, what, "keep is negative")
+
+
+def _attention_q8(what, q, k_off, v_off, k_pages, v_pages, block_table, row_seq, positions, slot_mapping, cu_rows, seg_start, seg0, n,
+                  rows_of_seg, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, scale, window, max_context, slopes, sinks,
+                  q_temp, rates, cap, keep):
+    fn = _q8_fn("cbis_attention_q8", [_P, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _P, _L, _P, _L,
+                                      _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _P, _P, _F, _I, _F, _I])
+    coef, every = q_temp if q_temp else (0.0, 0)
+    st = fn(_at(q), q.stride(0), k_off, v_off, _at(k_pages.codes), _at(k_pages.scales), _at(v_pages.codes), _at(v_pages.scales),
+            _at(block_table), block_table.shape[1], block_table.shape[0], k_pages.codes.shape[0], _at(row_seq), _at(positions),
+            _at(slot_mapping), _at(cu_rows), _at(seg_start), seg0, n, rows_of_seg, q.shape[0], _at(out), out.stride(0), _at(scratch),
+            scratch.numel(), _at(counters), counters.numel(), n_head, n_kv_head, head_dim, page_size, scale, window, max_context,
+            dtype_code(q.dtype), _stream(), _at(sinks), _at(slopes), _at(rates), coef, int(every), cap, keep)
+    _check(st, what, f"rows={q.shape[0]} heads={n_head}/{n_kv_head} head_dim={head_dim} page={page_size}")
+
+
+def paged_decode_q8(qkv, k_off, v_off, k_pages, v_pages, block_table, row_seq, positions, slot_mapping, out, scratch, counters, n_head,
+                    n_kv_head, head_dim, page_size, scale, window, max_context, slopes=None, sinks=None, q_temp=None, rates=None,
+                    cap: float = 0.0, keep: int = 0):
+    """Decode attention (one query per row, bfloat16 or float32) over an 8-bit cache; with ``k_off >= 0`` the current token's key and
+    value are taken from ``qkv``, quantised and stored by the same kernel.  No context is longer than ``max_context``.  Head sizes
+    that are multiples of 16 up to 256, any page size.  ``scratch``, ``counters``: ``attention_q8_scratch``.  ``window``, ``slopes``, ``sinks``,
+    ``q_temp``, ``rates``, ``cap``, ``keep``: as in ``paged_attention_generic``.  A row whose request is no row of the block table, or that sees no
+    key, gets zeros; a page number that the cache does not have is passed over."""
+    what = "paged_decode_q8"
+    rows = qkv.shape[0]
+    dtype_code(qkv.dtype)
+    _q8_attention_checks(what, qkv, k_pages, v_pages, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, slopes,
+                         sinks, rates, keep)
+    _q8_int32(what, "row_seq", row_seq, rows)
+    _q8_int32(what, "positions", positions, rows)
+    if k_off >= 0:
+        wide = n_kv_head * head_dim
+        _q8_need(v_off >= 0 and max(k_off, v_off) + wide <= qkv.shape[1], what, f"keys and values of {wide} do not lie in rows of {tuple(qkv.shape)}")
+        _q8_int32(what, "slot_mapping", slot_mapping, rows)
+    _q8_here(what, qkv, *k_pages, *v_pages, block_table, row_seq, positions, slot_mapping, out, scratch, counters, slopes, sinks, rates)
+    if rows == 0:
+        return
+    _attention_q8(what, qkv, k_off, v_off, k_pages, v_pages, block_table, row_seq, positions, slot_mapping, None, None, 0, rows, 0, out,
+                  scratch, counters, n_head, n_kv_head, head_dim, page_size, scale, int(window), int(max_context), slopes, sinks, q_temp,
+                  rates, float(cap), int(keep))
+
+
+def prefill_q8_reads_back(max_seg_rows: int, n_head: int, n_kv_head: int, head_dim: int, page_size: int, dtype, slopes=None, sinks=None,
+                          q_temp=None, rates=None, cap: float = 0.0, keep: int = 0) -> bool:
+    """Whether ``paged_prefill_q8`` reads the cache back first: chunks of many rows, for which a kernel over values is there."""
+    if max_seg_rows * (n_head // n_kv_head) <= 64 or page_size & (page_size - 1) or head_dim > 128:
+        return False
+    if dtype == torch.float32:
+        return slopes is None and sinks is None and q_temp is None and not cap and not keep
+    return True
+
+
+def paged_prefill_q8(q, k_pages, v_pages, block_table, cu_rows, seg_start, seg_ctx, positions, out, seg0, n_seg, row0, n_rows, max_seg_rows,
+                     n_head, n_kv_head, head_dim, page_size, scale, window, max_context, scratch, counters, work=None, slopes=None,
+                     sinks=None, q_temp=None, rates=None, cap: float = 0.0, keep: int = 0):
+    """Attention of chunks of new tokens over an 8-bit cache that holds their keys and values already: the requests seg0 ..
+    seg0 + n_seg - 1, whose rows (``row0`` .. ``row0 + n_rows - 1`` in all, at most ``max_seg_rows`` each) are ``cu_rows[s]`` .. ``cu_rows[s + 1] - 1`` at positions
+    from ``seg_start[s]`` to ``seg_ctx[s] - 1``; no context is longer than ``max_context``.  A few rows go through the kernel that reads codes;
+    for many (``prefill_q8_reads_back``) the cache is read back into ``work``, a pair of pages of q's type and the codes' shape, and
+    attended to there.  Without ``work`` the first takes all.  The rest as in ``paged_decode_q8``."""
+    what = "paged_prefill_q8"
+    dtype_code(q.dtype)
+    _q8_attention_checks(what, q, k_pages, v_pages, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, slopes,
+                         sinks, rates, keep)
+    _q8_need(seg0 >= 0 and n_seg >= 0 and seg0 + n_seg <= block_table.shape[0], what, f"requests {seg0}..{seg0 + n_seg} are not in the block table")
+    _q8_need(row0 >= 0 and n_rows >= 0 and row0 + n_rows <= q.shape[0], what, f"rows {row0}..{row0 + n_rows} are not in q")
+    _q8_int32(what, "cu_rows", cu_rows, seg0 + n_seg + 1)
+    _q8_int32(what, "seg_start", seg_start, seg0 + n_seg)
+    _q8_int32(what, "seg_ctx", seg_ctx, seg0 + n_seg)
+    _q8_int32(what, "positions", positions, row0 + n_rows)
+    if work is not None:
+        for o, p in zip(work, (k_pages, v_pages)):
+            _q8_need(o.dtype == q.dtype and o.shape == p.codes.shape and o.is_contiguous(), what, "work must be contiguous, of q's type and the codes' shape")
+    _q8_here(what, q, *k_pages, *v_pages, block_table, cu_rows, seg_start, seg_ctx, positions, out, scratch, counters, slopes, sinks, rates,
+             *(work or ()))
+    if n_seg == 0 or n_rows == 0 or max_seg_rows <= 0:
+        return
+    window, cap, keep = int(window), float(cap), int(keep)
+    if work is None or not prefill_q8_reads_back(max_seg_rows, n_head, n_kv_head, head_dim, page_size, q.dtype, slopes, sinks, q_temp, rates, cap, keep):
+        return _attention_q8(what, q, -1, -1, k_pages, v_pages, block_table, None, None, None, cu_rows, seg_start, seg0, n_seg,
+                             int(max_seg_rows), out, scratch, counters, n_head, n_kv_head, head_dim, page_size, scale, window,
+                             int(max_context), slopes, sinks, q_temp, rates, cap, keep)
+    k, v = work
+    segs = slice(seg0, seg0 + n_seg)
+    tokens = min(max_context, abs(window) + max_seg_rows) if window else max_context
+    kv_read_q8(k_pages, v_pages, k, v, block_table[segs], seg_start[segs], seg_ctx[segs], tokens, window, keep, whole_pages=True)
+    chunks = _prefill_q8_chunks(max_seg_rows, n_seg, n_head, head_dim, max_context, q.dtype)
+    args = (q, k, v, block_table, cu_rows, seg_start, out, seg0, n_seg, max_seg_rows, n_head, n_kv_head, head_dim, page_size, scale, window)
+    tail = (scratch, positions, row0, n_rows)
+    if q.dtype == torch.float32:
+        return paged_prefill_f32(*args, chunks, *tail)
+    tc5 = (head_dim in (64, 128) and 8 <= page_size <= 128 and USE_TCGEN05 and q_temp is None and (slopes is None) == (rates is None)
+           and not (rates is not None and (cap or keep)) and out.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0)
+    if tc5:
+        return paged_prefill_tc5(*args, chunks, *tail, sinks=sinks, slopes=slopes, rates=rates, cap=cap, keep=keep)
+    if head_dim in (64, 128):      # the other kernel's tiles have 64 rows: fewer chunks than it would take are fine
+        chunks = (1, 0)
+    extra = {} if slopes is None and sinks is None and q_temp is None and not cap and not keep else dict(
+        v_head_dim=head_dim, slopes=slopes, sinks=sinks, q_temp=q_temp, rates=rates, cap=cap, keep=keep)
+    return paged_prefill_bf16(*args, chunks, *tail, **extra)
 
 
 def _need_columns(q, out, n_head, v_heads, head_dim, v_head_dim):
