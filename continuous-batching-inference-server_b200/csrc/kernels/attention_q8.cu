@@ -20,7 +20,7 @@ int columns8(int hdp, int f32, long long queries) {
   const int nt = queries <= 8 ? 1 : (queries <= 16 ? 2 : 4);
   return nt < most ? nt : most;
 }
-int blocks_per_sm(int hdp, int nt, int f32) { return hdp == 256 ? 2 : (nt == 1 && !f32 ? 4 : (nt == 4 || f32 ? 2 : 3)); }
+int blocks_per_sm(int hdp, int nt) { return nt == 1 && hdp < 256 ? 3 : 2; }      // as Q8Shape::BLOCKS
 
 // rows_of_seg 0: decoding, `n` rows; else `n` requests of at most so many rows.
 Q8Plan q8_plan(int n, int rows_of_seg, int n_head, int n_kv_head, int hd, int f32, int max_context) {
@@ -33,8 +33,8 @@ Q8Plan q8_plan(int n, int rows_of_seg, int n_head, int n_kv_head, int hd, int f3
   p.rows_per = rows_of_seg ? 8 * p.nt / p.heads_per : 1;
   p.tiles_per_seg = rows_of_seg ? (rows_of_seg + p.rows_per - 1) / p.rows_per : 1;
   p.items = (long long)n * p.tiles_per_seg;
-  const long long unit = p.hdp <= 64 ? 128 : 64, pairs = p.items * n_kv_head * p.head_blocks;
-  const long long units = pairs * ((max_context + unit - 1) / unit + 1), slots = 148LL * blocks_per_sm(p.hdp, p.nt, f32);
+  const long long unit = 64, pairs = p.items * n_kv_head * p.head_blocks;
+  const long long units = pairs * ((max_context + unit - 1) / unit + 1), slots = 148LL * blocks_per_sm(p.hdp, p.nt);
   p.blocks = units < slots ? units : slots;
   p.floats = p.blocks * 2 * 8 * p.nt * (p.hdp + 2);
   p.counters = pairs;
@@ -69,9 +69,10 @@ CBIS_EXPORT int cbis_attention_q8(const void* q, int ld, int k_off, int v_off, v
   if (n <= 0) return CBIS_OK;
   if (dtype != CBIS_F32 && dtype != CBIS_BF16) return CBIS_ERR_BAD_DTYPE;
   if (hd <= 0 || hd > 256 || hd % 16 || ps <= 0 || n_kv_head <= 0 || n_head <= 0 || n_head % n_kv_head || max_blocks <= 0 || keep < 0 ||
-      num_pages < 0 || rows_of_seg < 0 || max_context < 0 || n_rows < 0 || (rows_of_seg && (seg0 < 0 || seg0 + n > n_seqs)) || (!rows_of_seg && n > n_rows))
+      num_pages <= 0 || rows_of_seg < 0 || rows_of_seg > Q8_MAX_POSITION || max_context < 0 || n_rows < 0 || (rows_of_seg && (seg0 < 0 || seg0 + n > n_seqs)) || (!rows_of_seg && n > n_rows))
     return CBIS_ERR_BAD_SIZE;
-  if ((long long)max_blocks * ps > 0x7fffff00LL || (long long)num_pages * ps > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
+  if ((long long)max_blocks * ps >= Q8_MAX_POSITION || (long long)num_pages * ps > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
+  if (window < -Q8_MAX_POSITION) return CBIS_ERR_BAD_SIZE;
   const int f32 = dtype == CBIS_F32, align = f32 ? 4 : 8;
   if (ld % align || (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15)) return CBIS_ERR_ALIGNMENT;
   const Q8Plan p = q8_plan(n, rows_of_seg, n_head, n_kv_head, hd, f32, max_context);
@@ -85,7 +86,10 @@ CBIS_EXPORT int cbis_attention_q8(const void* q, int ld, int k_off, int v_off, v
   a.n_rows = n_rows; a.ld = ld; a.out_ld = out_ld; a.k_off = k_off; a.v_off = v_off; a.max_blocks = max_blocks; a.num_pages = num_pages; a.n_seqs = n_seqs;
   a.seg0 = seg0; a.n_items = (int)p.items; a.tiles_per_seg = p.tiles_per_seg; a.n_head = n_head; a.n_kv_head = n_kv_head;
   a.heads_per = p.heads_per; a.head_blocks = p.head_blocks; a.rows_per = p.rows_per;
-  a.hd = hd; a.ps = ps; a.window = window; a.keep = keep; a.temp_every = temp_every; a.scale = scale; a.cap = cap; a.temp_coef = temp_coef;
+  a.hd = hd; a.ps = ps; a.ps_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (ps == 1 << i) a.ps_shift = i;
+  a.window = window; a.keep = keep; a.temp_every = temp_every; a.scale = scale; a.cap = cap; a.temp_coef = temp_coef;
   const bool ext = cap > 0.f || (keep > 0 && window != 0) || slopes || temp_every > 0;
   cudaStream_t st = (cudaStream_t)stream;
   switch (p.hdp) {

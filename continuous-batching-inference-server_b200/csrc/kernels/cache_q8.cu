@@ -11,28 +11,30 @@ namespace cbis {
 template <typename TT, int IT>
 __global__ void __launch_bounds__(128)
 kv_write_q8_kernel(const TT* qkv, int ld, int k_off, int v_off, int8_t* kc, float* ks, int8_t* vc, float* vs, const int* slot_mapping,
-                   int n_slots, long long n_rows, int heads, int hd, int hd_v, int ps, int lpr, int both) {
+                   int n_slots, unsigned n_rows, int heads, int hd, int hd_v, int ps, int lpr_shift, int both) {
   constexpr int E = 16 / sizeof(TT);
   pdl_trigger();
-  pdl_wait();
-  const int sub = threadIdx.x % lpr;
-  const long long unit = (long long)blockIdx.x * (128 / lpr) + threadIdx.x / lpr;      // token, key or value, head
-  const int per_token = heads << both;
+  const int lpr = 1 << lpr_shift, sub = threadIdx.x & (lpr - 1);
+  const unsigned unit = (blockIdx.x << (7 - lpr_shift)) + (threadIdx.x >> lpr_shift), per_token = heads << both;      // token, key or value, head
   const bool in_range = unit < n_rows;
-  const int token = in_range ? (int)(unit / per_token) : 0;
-  const int place = in_range ? (int)(unit % per_token) : 0;
-  const int which = place / heads, h = place % heads, width = which ? hd_v : hd;
+  const unsigned token = in_range ? unit / per_token : 0, place = in_range ? unit - token * per_token : 0;
+  const bool which = place >= (unsigned)heads;
+  const int h = which ? place - heads : place, width = which ? hd_v : hd;
+  const TT* src = qkv + (size_t)token * ld + (which ? v_off : k_off) + h * width;
+  pdl_wait();
   const int slot = in_range ? slot_mapping[token] : -1;
   const bool live = slot >= 0 && slot < n_slots;
-  const TT* src = qkv + (size_t)token * ld + (which ? v_off : k_off) + (size_t)h * width;
+  uint4 raw[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {      // beside the slot, not after it
+    const int at = (i * lpr + sub) * E;
+    raw[i] = in_range && at < width ? *reinterpret_cast<const uint4*>(src + at) : make_uint4(0, 0, 0, 0);
+  }
   float x[IT][E];
   unsigned top = 0;
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    const int at = (i * lpr + sub) * E;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (live && at < width) raw = *reinterpret_cast<const uint4*>(src + at);
-    const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+    const unsigned w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if constexpr (E == 8) {
@@ -54,15 +56,8 @@ kv_write_q8_kernel(const TT* qkv, int ld, int k_off, int v_off, int8_t* kc, floa
   for (int i = 0; i < IT; ++i) {
     const int at = (i * lpr + sub) * E;
     if (at >= width) continue;
-    unsigned out[E / 4];
-#pragma unroll
-    for (int e = 0; e < E / 4; ++e) {
-      out[e] = 0;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) out[e] |= (unsigned)(q8_code(x[i][4 * e + b], scale, inv) & 0xff) << (8 * b);
-    }
-    if constexpr (E == 8) *reinterpret_cast<uint2*>(dst + at) = make_uint2(out[0], out[1]);
-    else *reinterpret_cast<unsigned*>(dst + at) = out[0];
+    if constexpr (E == 8) *reinterpret_cast<uint2*>(dst + at) = make_uint2(q8_codes4(x[i], scale, inv), q8_codes4(x[i] + 4, scale, inv));
+    else *reinterpret_cast<unsigned*>(dst + at) = q8_codes4(x[i], scale, inv);
   }
   if (sub == 0) (which ? vs : ks)[row] = scale;
 }
@@ -93,13 +88,21 @@ kv_write_q8_any_kernel(const TT* qkv, int ld, int k_off, int v_off, int8_t* kc, 
   if (lane == 0) (which ? vs : ks)[row] = scale;
 }
 
-// grid (pages of a request that may be read, requests): a block takes one page of one request, keys and values of all heads.  N
-// codes (N output bytes = 16) to a thread and step, so that a warp's stores fill whole lines.
+// Four codes as numbers: with the sign bit turned round a code is u = code + 128, and 0x4b0000uu is 2^23 + u.
+__device__ __forceinline__ void q8_numbers(unsigned w, float* v) {
+  w ^= 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650 | i)) - 8388736.f;
+}
+
+// grid (pages of a request that may be read, requests, parts of a page): a block takes a part of the rows (head, token) of one page of
+// one request, of the keys and of the values.  A thread takes N codes (16 output bytes) of a row at a time, `lpr` threads (a power of
+// two) side by side a row, and asks for four rows before it uses one.
 template <typename TT, int N>
 __global__ void __launch_bounds__(256)
 kv_read_q8_kernel(const int8_t* kc, const float* ks, const int8_t* vc, const float* vs, TT* ko, TT* vo, const int* block_table, int max_blocks,
                   int num_pages, const int* seg_start, const int* seg_ctx, int heads, int hd, int hd_v, int ps, int window, int keep,
-                  int kept_blocks, int whole) {
+                  int kept_blocks, int whole, int lpr_shift) {
   pdl_trigger();
   pdl_wait();
   const int s = blockIdx.y, ctx = min(seg_ctx[s], max_blocks * ps);
@@ -110,34 +113,56 @@ kv_read_q8_kernel(const int8_t* kc, const float* ks, const int8_t* vc, const flo
     kept = (kept + ps - 1) / ps * ps;
   }
   // the pages of the kept first tokens come first, then those from `first` on (a page that both name is taken by the second)
-  const int block = (int)blockIdx.x < kept_blocks ? (int)blockIdx.x : first / ps + (int)blockIdx.x - kept_blocks;
-  if ((int)blockIdx.x < kept_blocks && (block * ps >= kept || block >= first / ps)) return;
-  if (block * ps >= ctx) return;
+  const int block = (int)blockIdx.x < kept_blocks ? (int)blockIdx.x : first / ps + (int)blockIdx.x - kept_blocks, j0 = block * ps;
+  if ((int)blockIdx.x < kept_blocks && (j0 >= kept || block >= first / ps)) return;
+  if (j0 >= ctx) return;
   const int page = block_table[(size_t)s * max_blocks + block];
   if (page < 0 || page >= num_pages) return;
+  const int hi = min(ps, ctx - j0), lo = j0 < kept ? 0 : max(first - j0, 0), n = hi - lo;
+  const float inv_n = 1.f / n;
+  const size_t row0 = (size_t)page * heads * ps;
+  const int lpr = 1 << lpr_shift, sub = threadIdx.x & (lpr - 1), rows = heads * n, step = (256 >> lpr_shift) * gridDim.z;
   for (int which = 0; which < 2; ++which) {
     if (which && vc == nullptr) break;
-    const int width = which ? hd_v : hd, per = width / N, units = heads * ps * per;
-    const size_t row0 = (size_t)page * heads * ps;
+    const int width = which ? hd_v : hd;
     const int8_t* src = (which ? vc : kc) + row0 * width;
     const float* scales = (which ? vs : ks) + row0;
     TT* dst = (which ? vo : ko) + row0 * width;
-#pragma unroll 4
-    for (int u = threadIdx.x; u < units; u += 256) {
-      const int row = u / per, j = block * ps + row % ps;
-      if (j >= ctx || (j < first && j >= kept)) continue;
-      const float scale = scales[row];
-      if constexpr (N == 1) {
-        from_f32(dst[u], (float)src[u] * scale);
-      } else if constexpr (N == 4) {
-        const char4 c = *reinterpret_cast<const char4*>(src + (size_t)u * 4);
-        *reinterpret_cast<float4*>(dst + (size_t)u * 4) = make_float4(c.x * scale, c.y * scale, c.z * scale, c.w * scale);
-      } else {
-        const uint2 c = *reinterpret_cast<const uint2*>(src + (size_t)u * 8);
-        float v[8];
+    for (int r0 = blockIdx.z * (256 >> lpr_shift) + (threadIdx.x >> lpr_shift); r0 < rows; r0 += 4 * step) {
+      int at[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)((e < 4 ? c.x : c.y) >> (8 * (e & 3))) * scale;
-        store8(dst + (size_t)u * 8, v);
+      for (int k = 0; k < 4; ++k) {
+        const int r = r0 + k * step, h = (int)((r + 0.5f) * inv_n), slot = lo + r - h * n, j = j0 + slot;      // r / n: exact below 2^22
+        at[k] = r < rows && (j >= first || j < kept) ? h * ps + slot : -1;
+      }
+      for (int c = sub * N; c < width; c += lpr * N) {
+        float scale[4];
+        uint2 raw[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (at[k] < 0) continue;
+          const int8_t* p = src + (size_t)at[k] * width + c;
+          scale[k] = scales[at[k]];
+          if constexpr (N == 8) raw[k] = *reinterpret_cast<const uint2*>(p);
+          else if constexpr (N == 4) raw[k].x = *reinterpret_cast<const unsigned*>(p);
+          else raw[k].x = (unsigned)(int)*p;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (at[k] < 0) continue;
+          TT* p = dst + (size_t)at[k] * width + c;
+          float v[8];
+          if constexpr (N == 1) {
+            from_f32(*p, (float)(int)raw[k].x * scale[k]);
+          } else {
+            q8_numbers(raw[k].x, v);
+            if constexpr (N == 8) q8_numbers(raw[k].y, v + 4);
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] *= scale[k];
+            if constexpr (N == 8) store8(p, v);
+            else *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+          }
+        }
       }
     }
   }
@@ -161,14 +186,14 @@ CBIS_EXPORT int cbis_kv_write_q8(const void* qkv, int ld, int k_off, int v_off, 
   cudaStream_t st = (cudaStream_t)stream;
   const bool vec = hd % E == 0 && (!both || hd_v % E == 0) && ld % E == 0 && k_off % E == 0 && (!both || v_off % E == 0) &&
                    widest <= 32 * 4 * E && !(((uintptr_t)qkv | (uintptr_t)kc | (uintptr_t)vc) & 15);
-  int lpr = 1;
-  while (lpr < 32 && lpr * E < widest) lpr *= 2;
+  int lpr = 1, shift = 0;
+  while (lpr < 32 && lpr * E < widest) lpr *= 2, ++shift;
   const int its = (widest + lpr * E - 1) / (lpr * E);
   const long long blocks = vec ? (n_rows + 128 / lpr - 1) / (128 / lpr) : (n_rows + 3) / 4;
-  if (blocks > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
+  if (n_rows > 0x7fffffffLL || blocks > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
 #define CBIS_WRITE(TT, IT)                                                                                                        \
   return (int)launch_pdl(kv_write_q8_kernel<TT, IT>, dim3((unsigned)blocks), dim3(128), 0, st, (const TT*)qkv, ld, k_off, v_off,  \
-                         (int8_t*)kc, (float*)ks, (int8_t*)vc, (float*)vs, slot_mapping, n_slots, n_rows, heads, hd, hd_v, ps, lpr, both)
+                         (int8_t*)kc, (float*)ks, (int8_t*)vc, (float*)vs, slot_mapping, n_slots, (unsigned)n_rows, heads, hd, hd_v, ps, shift, both)
 #define CBIS_WRITE_ANY(TT)                                                                                                        \
   return (int)launch_pdl(kv_write_q8_any_kernel<TT>, dim3((unsigned)blocks), dim3(128), 0, st, (const TT*)qkv, ld, k_off, v_off,  \
                          (int8_t*)kc, (float*)ks, (int8_t*)vc, (float*)vs, slot_mapping, n_slots, n_rows, heads, hd, hd_v, ps, both)
@@ -196,7 +221,8 @@ CBIS_EXPORT int cbis_kv_read_q8(const void* kc, const void* ks, const void* vc, 
   if (n_seg <= 0 || max_tokens <= 0) return CBIS_OK;
   if (hd_v <= 0) hd_v = hd;
   if (heads <= 0 || hd <= 0 || ps <= 0 || max_blocks <= 0 || keep < 0 || n_seg > 65535) return CBIS_ERR_BAD_SIZE;
-  if ((long long)max_blocks * ps > 0x7fffffffLL || (long long)heads * ps * (hd > hd_v ? hd : hd_v) > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
+  if (window < -(1 << 30)) return CBIS_ERR_BAD_SIZE;
+  if ((long long)max_blocks * ps >= 1 << 30 || (long long)heads * ps * (hd > hd_v ? hd : hd_v) > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
   if (dtype != CBIS_F32 && dtype != CBIS_BF16) return CBIS_ERR_BAD_DTYPE;
   const int kept_blocks = window != 0 ? (keep + ps - 1) / ps : 0;
   long long blocks = (long long)(max_tokens - 1) / ps + 2;
@@ -207,11 +233,21 @@ CBIS_EXPORT int cbis_kv_read_q8(const void* kc, const void* ks, const void* vc, 
   const bool vec = hd % N == 0 && (!vc || hd_v % N == 0) &&
                    !(((uintptr_t)kc | (uintptr_t)vc | (uintptr_t)ko | (uintptr_t)vo) & 15);
   cudaStream_t st = (cudaStream_t)stream;
-  const dim3 grid((unsigned)blocks, n_seg);
+  int shift = 0;
+  const int widest = vc && hd_v > hd ? hd_v : hd;
+  while (shift < 5 && (vec ? N : 1) << shift < widest) ++shift;
+  // parts of a page: four rows to a thread if there are blocks enough, fewer rows for a few pages
+  const long long rows = (long long)heads * ps, per_block = 256 >> shift, pages = blocks * n_seg;
+  long long parts = (rows + 4 * per_block - 1) / (4 * per_block), finest = (rows + per_block - 1) / per_block;
+  if (pages * parts < 4 * 148) parts = (4 * 148 + pages - 1) / pages;
+  if (parts > finest) parts = finest;
+  if (parts > 65535) parts = 65535;
+  if (rows > 1 << 22) return CBIS_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)blocks, n_seg, (unsigned)parts);
 #define CBIS_READ(TT, NN)                                                                                                              \
   return (int)launch_pdl(kv_read_q8_kernel<TT, NN>, grid, dim3(256), 0, st, (const int8_t*)kc, (const float*)ks, (const int8_t*)vc,    \
                          (const float*)vs, (TT*)ko, (TT*)vo, block_table, max_blocks, num_pages, seg_start, seg_ctx, heads, hd, hd_v, \
-                         ps, window, keep, kb, whole)
+                         ps, window, keep, kb, whole, shift)
   if (dtype == CBIS_F32) {
     if (vec) CBIS_READ(float, 4);
     CBIS_READ(float, 1);

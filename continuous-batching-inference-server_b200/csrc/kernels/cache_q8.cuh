@@ -18,7 +18,28 @@ __device__ __forceinline__ float q8_scale(unsigned amax_bits) {
   return amax_bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__fdiv_rn(__uint_as_float(amax_bits), 127.f), Q8_FLOOR);
 }
 
-// inv: the reciprocal of the scale.  q is at most one step off; the remainder x - q scale is exact in 32 bits.
+// The codes of four numbers, a byte each.  Adding 1.5 * 2^23 rounds x / scale to a whole number, ties to even, and leaves it in the low
+// bits; the quotient is a product with the reciprocal, good to 2^-22, so only a number that close to a half step needs the exact way.
+__device__ __forceinline__ int q8_code(float x, float scale, float inv);
+__device__ __forceinline__ unsigned q8_codes4(const float* x, float scale, float inv) {
+  float f[4];
+  bool close = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float y = x[i] * inv;
+    f[i] = y + 12582912.f;
+    close |= fabsf(y - (f[i] - 12582912.f)) > 0.4999f;
+  }
+  if (close) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = (float)q8_code(x[i], scale, inv) + 12582912.f;
+  }
+  const unsigned w = __byte_perm(__byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x0040),
+                                 __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0040), 0x5410);
+  return scale == scale ? w : 0u;
+}
+
+// The same one by one.  inv: the reciprocal of the scale.  q is at most one step off; the remainder x - q scale is exact in 32 bits.
 __device__ __forceinline__ int q8_code(float x, float scale, float inv) {
   float q = rintf(x * inv);
   const float r = fmaf(-q, scale, x), half = 0.5f * scale;
