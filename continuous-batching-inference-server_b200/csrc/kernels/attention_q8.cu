@@ -20,7 +20,7 @@ int columns8(int hdp, int f32, long long queries) {
   const int nt = queries <= 8 ? 1 : (queries <= 16 ? 2 : 4);
   return nt < most ? nt : most;
 }
-int blocks_per_sm(int hdp, int nt) { return nt == 1 && hdp < 256 ? 3 : 2; }      // as Q8Shape::BLOCKS
+int blocks_per_sm(int hdp, int nt, int f32) { return nt == 1 && hdp < 256 ? (f32 ? 3 : 4) : 2; }      // as Q8Shape::BLOCKS
 
 // rows_of_seg 0: decoding, `n` rows; else `n` requests of at most so many rows.
 Q8Plan q8_plan(int n, int rows_of_seg, int n_head, int n_kv_head, int hd, int f32, int max_context) {
@@ -30,11 +30,21 @@ Q8Plan q8_plan(int n, int rows_of_seg, int n_head, int n_kv_head, int hd, int f3
   p.nt = columns8(p.hdp, f32, (long long)group * (rows_of_seg ? rows_of_seg : 1));
   p.heads_per = group < 8 * p.nt ? group : 8 * p.nt;
   p.head_blocks = (group + p.heads_per - 1) / p.heads_per;
-  p.rows_per = rows_of_seg ? 8 * p.nt / p.heads_per : 1;
-  p.tiles_per_seg = rows_of_seg ? (rows_of_seg + p.rows_per - 1) / p.rows_per : 1;
+  const long long rows = rows_of_seg ? rows_of_seg : 1, fit = 8 * p.nt / p.heads_per;
+  p.rows_per = (int)(rows < fit ? rows : fit);
+  p.tiles_per_seg = (int)((rows + p.rows_per - 1) / p.rows_per);
   p.items = (long long)n * p.tiles_per_seg;
-  const long long unit = 64, pairs = p.items * n_kv_head * p.head_blocks;
-  const long long units = pairs * ((max_context + unit - 1) / unit + 1), slots = 148LL * blocks_per_sm(p.hdp, p.nt);
+  if (p.items > Q8_MAX_ITEMS) return p;
+  // three stages a warp where that many blocks still fit on an SM, else two
+  const int stage = (p.hdp >= 128 ? 1 : 128 / p.hdp) * (32 * p.hdp + 128), ldq = p.hdp >= 128 ? p.hdp + 16 : p.hdp;
+  int fit_blocks = blocks_per_sm(p.hdp, p.nt, f32);
+  for (p.stages = 3;; p.stages = 2) {
+    p.smem = q8_smem(stage, p.hdp + 8, ldq, p.stages, p.rows_per * p.heads_per, (int)p.items).bytes;
+    if (fit_blocks * (p.smem + 1024) <= 228 * 1024 || p.stages == 2) break;
+  }
+  while (fit_blocks > 1 && fit_blocks * (p.smem + 1024) > 228 * 1024) --fit_blocks;
+  const long long unit = 64 * (p.hdp >= 128 ? 1 : 128 / p.hdp), pairs = p.items * n_kv_head * p.head_blocks;
+  const long long units = pairs * ((max_context + unit - 1) / unit + 1), slots = 148LL * fit_blocks;
   p.blocks = units < slots ? units : slots;
   p.floats = p.blocks * 2 * 8 * p.nt * (p.hdp + 2);
   p.counters = pairs;
@@ -71,12 +81,12 @@ CBIS_EXPORT int cbis_attention_q8(const void* q, int ld, int k_off, int v_off, v
   if (hd <= 0 || hd > 256 || hd % 16 || ps <= 0 || n_kv_head <= 0 || n_head <= 0 || n_head % n_kv_head || max_blocks <= 0 || keep < 0 ||
       num_pages <= 0 || rows_of_seg < 0 || rows_of_seg > Q8_MAX_POSITION || max_context < 0 || n_rows < 0 || (rows_of_seg && (seg0 < 0 || seg0 + n > n_seqs)) || (!rows_of_seg && n > n_rows))
     return CBIS_ERR_BAD_SIZE;
-  if ((long long)max_blocks * ps >= Q8_MAX_POSITION || (long long)num_pages * ps > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
+  if ((long long)max_blocks * ps >= Q8_MAX_POSITION || (long long)num_pages * ps * n_kv_head > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
   if (window < -Q8_MAX_POSITION) return CBIS_ERR_BAD_SIZE;
   const int f32 = dtype == CBIS_F32, align = f32 ? 4 : 8;
   if (ld % align || (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15)) return CBIS_ERR_ALIGNMENT;
   const Q8Plan p = q8_plan(n, rows_of_seg, n_head, n_kv_head, hd, f32, max_context);
-  if (p.items > Q8_MAX_ITEMS) return CBIS_ERR_TOO_LARGE;
+  if (p.items > Q8_MAX_ITEMS || p.items * ((long long)max_blocks * ps / 64 + 3) > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;      // the units are counted in 32 bits
   if (part_floats < p.floats || n_counters < p.counters || (k_off >= 0 && slot_mapping == nullptr)) return CBIS_ERR_BAD_SIZE;
   Q8Args a = {};
   a.q = q; a.out = out; a.kc = (int8_t*)kc; a.vc = (int8_t*)vc; a.ks = (float*)ks; a.vs = (float*)vs;
@@ -86,7 +96,7 @@ CBIS_EXPORT int cbis_attention_q8(const void* q, int ld, int k_off, int v_off, v
   a.n_rows = n_rows; a.ld = ld; a.out_ld = out_ld; a.k_off = k_off; a.v_off = v_off; a.max_blocks = max_blocks; a.num_pages = num_pages; a.n_seqs = n_seqs;
   a.seg0 = seg0; a.n_items = (int)p.items; a.tiles_per_seg = p.tiles_per_seg; a.n_head = n_head; a.n_kv_head = n_kv_head;
   a.heads_per = p.heads_per; a.head_blocks = p.head_blocks; a.rows_per = p.rows_per;
-  a.hd = hd; a.ps = ps; a.ps_shift = -1;
+  a.stages = p.stages; a.page_rows = n_kv_head * ps; a.hd = hd; a.ps = ps; a.ps_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (ps == 1 << i) a.ps_shift = i;
   a.window = window; a.keep = keep; a.temp_every = temp_every; a.scale = scale; a.cap = cap; a.temp_coef = temp_coef;

@@ -12,20 +12,25 @@
 //
 // Both products are taken with the operands swapped, keys and values as the 16-row operand and the queries as the 8 columns:
 // S^T = K Q^T, O^T = V^T P^T.  The query heads that share a key/value head, and a chunk's rows, are the columns, so up to 8 of them cost
-// what one does.  A lane loads 16-byte pieces of its two keys (K) and of its four keys (V); the order of the contraction, and that of
-// the output's rows, is free, so the pieces are fragments as they come, without shared memory.
+// what one does.  The order of the contraction, and that of the output's rows, is free: a lane's share of the values is 16-byte pieces of its four keys.  They come through shared memory, a ring of stages for every warp alone, which it fills with
+// 16-byte asynchronous copies and reads without two lanes on one bank (q8_place): what is on its way holds no registers, so four
+// blocks fit on an SM, and a block asks for the first tiles of its next piece before it finishes the one in hand.
 //
-// The keys of all (row, head) pairs are one row of units (64 or 128 keys), which is cut evenly over the blocks: every block works out
-// its part from the positions on the device.  A pair that lies in several blocks is merged by the last one to finish it.
+// The keys of all (row, head) pairs are one row of units (16 KB of codes, and one more for what a pair costs beside them), which is cut
+// evenly over the blocks: every block works out its part from the positions on the device.  A cut that would leave a short end of a
+// pair is moved to the pair's end: a pair that lies in several blocks is merged by the last one to finish it, which takes as long as
+// some three units.
 #pragma once
 #include "cache_q8.cuh"
 #include "mma_sync.cuh"
+#include <atomic>
 #include <math.h>
 #include <type_traits>
 
 namespace cbis {
 
 constexpr int Q8_WARPS = 4, Q8_THREADS = Q8_WARPS * 32, Q8_MAX_ITEMS = 4096;
+constexpr int Q8_PAIR = 1, Q8_MERGE = 3;      // what a pair and a merge cost, in units
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Q8Args {
@@ -38,7 +43,7 @@ struct Q8Args {
   unsigned* counters;
   const float *sinks, *slopes, *rates;
   int n_rows, ld, out_ld, k_off, v_off, max_blocks, num_pages, n_seqs, seg0, n_items, tiles_per_seg, n_head, n_kv_head, heads_per, head_blocks, rows_per;
-  int hd, ps, ps_shift, window, keep, temp_every;      // ps_shift: log2 of the page size, -1 where that is no whole number
+  int stages, page_rows, hd, ps, ps_shift, window, keep, temp_every;      // ps_shift: log2 of the page size, -1 where that is no whole number
   float scale, cap, temp_coef;
 };
 
@@ -83,9 +88,11 @@ __device__ __forceinline__ Q8Span q8_span(const Q8Args& a, const Q8Item& it) {
 }
 
 // The two bytes of `w` that hold signed codes (byte 0 and byte 2; the others are anything) as two bfloat16: 128 + the low seven bits,
-// less 128 or 256 as the sign bit says.
-__device__ __forceinline__ unsigned q8_pair(unsigned w) {
-  const unsigned low = (w & 0x007f007fu) | 0x43004300u, off = (w & 0x00800080u) | 0x43004300u;
+// less 128 or 256 as the sign bit says.  `base`: 0x43004300 from a register, or each of the two would be two instructions.
+__device__ __forceinline__ unsigned q8_pair(unsigned w, unsigned base) {
+  unsigned low, off;
+  asm("lop3.b32 %0, %1, 0x007f007f, %2, 0xea;" : "=r"(low) : "r"(w), "r"(base));      // (w & mask) | base
+  asm("lop3.b32 %0, %1, 0x00800080, %2, 0xea;" : "=r"(off) : "r"(w), "r"(base));
   const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&low), *reinterpret_cast<const __nv_bfloat162*>(&off));
   return *reinterpret_cast<const unsigned*>(&r);
 }
@@ -93,6 +100,11 @@ __device__ __forceinline__ void mma_16832_s8(int (&c)[4], const unsigned (&a)[4]
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_16832_s8_first(int (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {      // c = the product
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
 }
 __device__ __forceinline__ unsigned transposed(unsigned v) {      // an 8 x 8 tile of 16-bit numbers, a row to four lanes
   unsigned r;
@@ -105,59 +117,118 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-__device__ __forceinline__ float load_float(const float* p) {
+__device__ __forceinline__ float load_float(const float* p) {      // what another block may have written
   float r;
   asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(r) : "l"(p) : "memory");
   return r;
 }
-template <int HDP>
-struct Q8Lane {                       // what a lane loads of a key: PIECES pieces of WORDS words; of a value: VWORDS words in a row
-  static constexpr int WORDS = HDP >= 64 ? 4 : 2, PIECES = HDP / (16 * WORDS), VWORDS = HDP / 32;
-};
-template <int WORDS>
-__device__ __forceinline__ void load_words(unsigned* r, const int8_t* p) {
-  if constexpr (WORDS == 1) {
-    asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(r[0]) : "l"(p) : "memory");
-  } else if constexpr (WORDS == 2) {
-    asm volatile("ld.global.cg.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p) : "memory");
-  } else {
-    asm volatile("ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "l"(p) : "memory");
-  }
+// Asynchronous copies to shared memory; of 16 bytes, or of none and zeros instead.
+__device__ __forceinline__ void copy16(unsigned to, const void* from, bool ok) {
+  const int n = ok ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
 }
+__device__ __forceinline__ void copy16(unsigned to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void copy4(unsigned to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Where byte `byte` of the row of key `row` (0..15) lies in a tile of rows of HDP bytes: the 16-byte pieces of a 128-byte line are
+// exchanged by the row's number, so that the same piece of eight keys (ldmatrix), and the pieces that eight lanes read of keys 2t,
+// lie on different banks.
+template <int HDP>
+__device__ __forceinline__ int q8_place(int row, int byte) {
+  const int at = row * HDP + byte;
+  if constexpr (HDP == 128) return at ^ ((row & 7) << 4);
+  if constexpr (HDP == 64) return at ^ ((((row >> 1) & 3) | ((row & 2) << 1)) << 4);
+  if constexpr (HDP == 32) return at ^ ((row >> 2 & 1) * 48);
+  return at ^ (((row & 4) | ((row >> 1) & 1) | ((row & 1) << 1)) << 4);
+}
+template <int WORDS>
+__device__ __forceinline__ void read_words(unsigned* r, unsigned at) {
+  if constexpr (WORDS == 1) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(at) : "memory");
+  else if constexpr (WORDS == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at) : "memory");
+  else asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ float read_float(unsigned at) {
+  float r;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(at) : "memory");
+  return r;
+}
+// The bytes 32 x .. 32 x + 31 of 16 keys as the A fragment of a product on signed bytes, from a lane's share of the addresses.
+__device__ __forceinline__ void read_keys(unsigned (&r)[4], unsigned at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+// What q8_place adds to a lane's first place, as an exchange of address bits and a distance: 32 bytes x further in a row, for key 2t + 1
+// instead of 2t, and for step i of a copy (32 pieces of 16 bytes a step).
+template <int HDP>
+struct Q8Place {
+  static __device__ __forceinline__ unsigned key(unsigned at, int x) { return (at ^ ((x & 3) * 32)) + (x >> 2) * 128; }
+  static __device__ __forceinline__ unsigned odd(unsigned at) {
+    return HDP == 256 ? (at ^ 32) + 256 : (HDP == 128 ? (at ^ 16) + 128 : at ^ (HDP == 64 ? 64 : 32));
+  }
+  static __device__ __forceinline__ unsigned copy(unsigned at, int i) {
+    return (HDP == 256 ? at ^ ((i & 1 ? 16 : 0) | (i & 2 ? 64 : 0)) : (HDP == 128 ? at ^ (i & 1 ? 64 : 0) : at)) + i * 512;
+  }
+};
 
 // HDP: the width rounded up to 32, 64, 128 or 256; NT: columns of queries / 8; PARTS: bfloat16 parts of a weight (1: bfloat16 rows, 3:
 // 32-bit rows); EXT: kept first keys, a cap, a distance bias, a query temperature; FAST: the width is HDP and pages are a multiple of 16 keys.
 template <int HDP, int NT, int PARTS>
 struct Q8Shape {
-  static constexpr int TPW = HDP * NT <= 32 ? 4 : (HDP * NT <= 128 ? 2 : 1);      // tiles a warp takes through one update of its maxima and sums
-  static constexpr int UNIT = Q8_WARPS * TPW;                                     // tiles of a unit
+  static constexpr int TPW = HDP >= 128 ? 1 : 128 / HDP;        // tiles a warp takes through one update of its maxima and sums: a stage of its ring
+  static constexpr int UNIT = Q8_WARPS * TPW;                   // tiles of a unit
   static constexpr int NQ = 8 * NT;
-  static constexpr int LDS = HDP + 8;                                             // floats of a query's sums in shared memory
-  static constexpr int LDQ = HDP >= 128 ? HDP + 64 : HDP;                         // bytes of a query's row in shared memory: no two lanes of a load on one bank
-  static constexpr int BLOCKS = NT == 1 && HDP < 256 ? 3 : 2;                     // per SM
-  static constexpr int FLOATS = Q8_WARPS * NQ * (LDS + 2) + 3 * NQ + 8;
-  static size_t smem(int n_items) { return (size_t)FLOATS * 4 + 3 * NQ * LDQ + (size_t)(n_items + 1) * 4; }
+  static constexpr int LDS = HDP + 8;                           // floats of a query's sums in shared memory
+  static constexpr int LDQ = HDP >= 128 ? HDP + 16 : HDP;       // bytes of a query's row in shared memory: no two lanes of a load on one bank
+  static constexpr int TILE = 32 * HDP + 128;                   // bytes of 16 keys: codes of keys, of values, their scales
+  static constexpr int STAGE = TPW * TILE;
+  static constexpr int BLOCKS = NT == 1 && HDP < 256 ? (PARTS == 1 ? 4 : 3) : 2;      // per SM, as far as registers go
 };
+// Shared memory of a block (in this order): the warps' rings; sums, maxima of up to 8 columns from four warps; the queries' bytes; the
+// columns' powers of two, merged maxima and sums; a few integers; the items.
+struct Q8Smem {
+  int ring, join, stats, queries, columns, ints, items, bytes;
+};
+__host__ __device__ inline Q8Smem q8_smem(int stage, int lds, int ldq, int stages, int live, int n_items) {
+  Q8Smem s;
+  const int jq = live < 8 ? live : 8;
+  s.ring = 0;
+  s.join = Q8_WARPS * stages * stage;
+  s.stats = s.join + Q8_WARPS * jq * lds * 4;
+  s.queries = s.stats + Q8_WARPS * 8 * 2 * 4;
+  s.columns = s.queries + 3 * live * ldq;
+  s.ints = s.columns + 3 * 32 * 4;
+  s.items = s.ints + 32;
+  s.bytes = s.items + (4 * n_items + 1) * 4;
+  return s;
+}
 
 template <int HDP, int NT, int PARTS, bool EXT, bool FAST>
 __global__ void __launch_bounds__(Q8_THREADS, Q8Shape<HDP, NT, PARTS>::BLOCKS)
 attention_q8_kernel(const __grid_constant__ Q8Args a) {
   using Shape = Q8Shape<HDP, NT, PARTS>;
-  using Lane = Q8Lane<HDP>;
   using TT = typename std::conditional<PARTS == 1, __nv_bfloat16, float>::type;
   constexpr int TPW = Shape::TPW, UNIT = Shape::UNIT, NQ = Shape::NQ, LDS = Shape::LDS, LDQ = Shape::LDQ, KS = HDP / 16;
-  constexpr int W = Lane::WORDS, PIECES = Lane::PIECES, VW = Lane::VWORDS;
+  constexpr int STEPS = HDP / 32, VW = HDP / 32, PW = VW < 4 ? VW : 4;      // steps of the scores' product; words of a value that a lane takes, of one load
   constexpr bool Q_IN_REGS = NT * HDP <= 128;
-  extern __shared__ __align__(16) float sm[];
-  float* sm_acc = sm;                                   // [warp][NQ][LDS]
-  float* sm_m = sm_acc + Q8_WARPS * NQ * LDS;           // [warp][NQ]
-  float* sm_l = sm_m + Q8_WARPS * NQ;                   // [warp][NQ]
-  float* sm_w = sm_l + Q8_WARPS * NQ;                   // [NQ] maximum, [NQ] sum of the merged pieces
-  float* sm_f = sm_w + 2 * NQ;                          // [NQ] a query's power of two
-  int* sm_i = reinterpret_cast<int*>(sm_f + NQ);        // [8]
-  int8_t* sm_q = reinterpret_cast<int8_t*>(sm + Shape::FLOATS);      // [3][NQ][LDQ] the queries' bytes, the highest first
-  int* before = reinterpret_cast<int*>(sm_q + 3 * NQ * LDQ);         // [n_items + 1] units of the items before this one
+  extern __shared__ __align__(128) char smem[];
+  const int cols = a.rows_per * a.heads_per;            // live columns at most
+  const Q8Smem at = q8_smem(Shape::STAGE, LDS, LDQ, a.stages, cols, a.n_items);
+  float* sm_acc = reinterpret_cast<float*>(smem + at.join);          // [warp][min(cols, 8)][LDS]
+  float* sm_m = reinterpret_cast<float*>(smem + at.stats);           // [warp][8]
+  float* sm_l = sm_m + Q8_WARPS * 8;                                 // [warp][8]
+  int8_t* sm_q = reinterpret_cast<int8_t*>(smem + at.queries);       // [3][cols][LDQ] the queries' bytes, the highest first
+  float* sm_f = reinterpret_cast<float*>(smem + at.columns);         // [32] a query's power of two, [32] maximum and [32] sum of merged pieces
+  float* sm_w = sm_f + 32;
+  int* sm_i = reinterpret_cast<int*>(smem + at.ints);                // [8]
+  int* before = reinterpret_cast<int*>(smem + at.items);             // [n_items + 1] units of the items before this one
+  int* item_row = before + a.n_items + 1;                            // [n_items] first row; request or rows; first position
+  int* item_seq = item_row + a.n_items;
+  int* item_pos = item_seq + a.n_items;
   const int hd = FAST ? HDP : a.hd;
+  unsigned base;
+  asm volatile("mov.b32 %0, 0x43004300;" : "=r"(base));
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -169,7 +240,10 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
     int n = 0;
     if (i < a.n_items) {
       const Q8Item it = q8_item(a, i);
-      if (it.n_rows > 0) n = max((q8_span<EXT>(a, it).tiles + UNIT - 1) / UNIT, 1);      // a row without keys has its zeros written too
+      if (it.n_rows > 0) n = Q8_PAIR + (q8_span<EXT>(a, it).tiles + UNIT - 1) / UNIT;      // a row without keys has its zeros written too
+      item_row[i] = it.row0;
+      item_seq[i] = a.cu_rows ? it.n_rows : it.seq;
+      item_pos[i] = it.pos0;
     }
     int sum = n;
 #pragma unroll
@@ -179,43 +253,91 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
     }
     if (lane == 31) sm_i[warp] = sum;
     __syncthreads();
-    int at = total;
+    int sofar = total;
 #pragma unroll
     for (int w = 0; w < Q8_WARPS; ++w) {
-      if (w < warp) at += sm_i[w];
+      if (w < warp) sofar += sm_i[w];
       total += sm_i[w];
     }
-    if (i < a.n_items) before[i] = at + sum - n;
+    if (i < a.n_items) before[i] = sofar + sum - n;
     __syncthreads();
   }
   if (tid == 0) before[a.n_items] = total;
   __syncthreads();
-  const int n_hg = a.n_kv_head * a.head_blocks;
-  const long long all = (long long)total * n_hg, per = (all + gridDim.x - 1) / gridDim.x;
-  const long long w_end = min(all, (blockIdx.x + 1) * per);
-
-  for (long long w_at = blockIdx.x * per; w_at < w_end;) {
-    const int hg = (int)(w_at / total), rem = (int)(w_at % total);
-    int lo = 0, hi = a.n_items - 1;                    // the last item that begins at or before rem
+  const int n_hg = a.n_kv_head * a.head_blocks, group = a.n_head / a.n_kv_head;
+  if (total == 0) return;
+  const long long all = (long long)total * n_hg, per = max((all + gridDim.x - 1) / gridDim.x, (long long)Q8_MERGE);
+  const int slack = (int)min(per - 1, (long long)Q8_MERGE);
+  // the item in which unit `rem` of a head lies: the last one that begins at or before it
+  auto item_at = [&](int rem) {
+    int lo = 0, hi = a.n_items - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (before[mid] <= rem) lo = mid; else hi = mid - 1;
     }
-    const int item = lo, units = before[item + 1] - before[item], u0 = rem - before[item];
-    const int u1 = (int)min((long long)units, u0 + (w_end - w_at));
-    const Q8Item it = q8_item(a, item);
-    const Q8Span span = q8_span<EXT>(a, it);
-    const int hk = hg / a.head_blocks, hb = hg % a.head_blocks, group = a.n_head / a.n_kv_head;
-    const int h0 = hk * group + hb * a.heads_per, n_h = min(a.heads_per, group - hb * a.heads_per), live = it.n_rows * n_h;
-    const int* bt = a.block_table + (size_t)max(it.seq, 0) * a.max_blocks;
-    const int last = it.pos0 + it.n_rows - 1;
-    const int end_tile = min(u1 * UNIT, span.tiles);
+    return lo;
+  };
+  auto cut = [&](long long x) {      // a block's end, moved to that of an item that is near
+    if (x >= all) return all;
+    const int rem = (int)(x % total), i = item_at(rem), d = rem - before[i], e = before[i + 1] - rem;
+    return d <= slack ? x - d : (e <= slack ? x + e : x);
+  };
+  long long w_at = cut(blockIdx.x * per);
+  const long long w_end = cut((blockIdx.x + 1) * per);
+  if (w_at >= w_end) return;
 
+  // A block's part of one item's keys under the heads that share a key/value head: units u0 .. u1 - 1.
+  struct Piece {
+    Q8Item it;
+    Q8Span span;
+    int hg, hk, h0, n_h, item, u0, u1, end_tile;
+    bool begins, ends;      // whether the item does with it
+    const int* bt;
+    const int8_t *k_lane, *v_lane;      // FAST: the lane's piece of the head's first row, and its scale
+    const float* s_lane;
+  };
+  int at_hg = (int)(w_at / total), at_item = item_at((int)(w_at % total)), at_unit = (int)(w_at % total) - before[at_item];
+  auto find_piece = [&](Piece& p) {
+    const int lo = at_item, slots = before[lo + 1] - before[lo], to = (int)min((long long)slots, at_unit + (w_end - w_at));
+    p.hg = at_hg;
+    p.item = lo;
+    p.begins = at_unit == 0;
+    p.ends = to == slots;
+    p.u0 = p.begins ? 0 : at_unit - Q8_PAIR;
+    p.u1 = max(to - Q8_PAIR, 0);
+    w_at += to - at_unit;
+    at_unit = to;
+    if (p.ends) {
+      at_unit = 0;
+      do {
+        if (++at_item == a.n_items) {
+          at_item = 0;
+          ++at_hg;
+        }
+      } while (w_at < w_end && before[at_item + 1] == before[at_item]);
+    }
+    p.it.row0 = item_row[lo];
+    p.it.pos0 = item_pos[lo];
+    p.it.n_rows = a.cu_rows ? item_seq[lo] : 1;
+    p.it.seq = a.cu_rows ? a.seg0 + lo / a.tiles_per_seg : item_seq[lo];
+    p.span = q8_span<EXT>(a, p.it);
+    p.hk = a.head_blocks == 1 ? p.hg : p.hg / a.head_blocks;
+    const int hb = p.hg - p.hk * a.head_blocks;
+    p.h0 = p.hk * group + hb * a.heads_per;
+    p.n_h = min(a.heads_per, group - hb * a.heads_per);
+    p.bt = a.block_table + (size_t)max(p.it.seq, 0) * a.max_blocks;
+    p.end_tile = min(p.u1 * UNIT, p.span.tiles);
+    if constexpr (FAST) {
+      const long long first = (long long)p.hk * a.ps;
+      p.k_lane = a.kc + first * HDP + lane * 16;
+      p.v_lane = a.vc + first * HDP + lane * 16;
+      p.s_lane = (lane < 16 ? a.ks : a.vs) + first + (lane & 15);
+    }
     // the current token's key and value are stored by the block that reads them
-    if (a.k_off >= 0 && u1 == units && it.seq >= 0) {
-      const int slot = a.slot_mapping[it.row0];
+    if (a.k_off >= 0 && p.ends && p.it.seq >= 0) {
+      const int slot = a.slot_mapping[p.it.row0];
       if (slot >= 0 && slot < a.num_pages * a.ps && warp < 2) {
-        const TT* src = static_cast<const TT*>(a.q) + (size_t)it.row0 * a.ld + (warp ? a.v_off : a.k_off) + hk * hd;
+        const TT* src = static_cast<const TT*>(a.q) + (size_t)p.it.row0 * a.ld + (warp ? a.v_off : a.k_off) + p.hk * hd;
         float x[HDP / 32];
         unsigned top = 0;
 #pragma unroll
@@ -226,24 +348,103 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         const float s = q8_scale(top), inv = 1.f / s;
-        const size_t row = ((size_t)(slot / a.ps) * a.n_kv_head + hk) * a.ps + slot % a.ps;
+        const size_t row = ((size_t)(slot / a.ps) * a.n_kv_head + p.hk) * a.ps + slot % a.ps;
         int8_t* dst = (warp ? a.vc : a.kc) + row * hd;
 #pragma unroll
         for (int i = 0; i < HDP / 32; ++i)
           if (i * 32 + lane < hd) dst[i * 32 + lane] = (int8_t)q8_code(x[i], s, inv);
         if (lane == 0) (warp ? a.vs : a.ks)[row] = s;
       }
+      __threadfence();
       __syncthreads();
     }
+  };
 
+  // The warp's ring: `fill` is the stage to be filled next, `use` the one to be read next (as shared addresses).
+  const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * a.stages * Shape::STAGE, ring_end = ring + a.stages * Shape::STAGE;
+  unsigned fill = ring, use = ring;
+  const unsigned k_place = q8_place<HDP>((lane & 7) + (lane & 8), lane >> 4 << 4), v_place = q8_place<HDP>(2 * t, g * 4 * VW) + 16 * HDP;
+  const unsigned c_place = q8_place<HDP>(lane / (HDP / 16), lane % (HDP / 16) * 16);
+  auto real_tile = [&](const Piece& p, int n) { return !EXT || n >= p.span.nk ? n + p.span.skipped : n; };
+  int ahead[TPW];                          // FAST: the pages of the tiles to be asked for next, as the table names them
+  auto find_pages = [&](const Piece& p, int tile) {
+#pragma unroll
+    for (int u = 0; u < TPW; ++u) {
+      const int j0 = real_tile(p, min(tile + u, p.end_tile - 1)) << 4;
+      ahead[u] = p.bt[a.ps_shift >= 0 ? j0 >> a.ps_shift : j0 / a.ps];
+    }
+  };
+  // Asks for the warp's tiles from `tile` on, as far as they lie in the piece.  A key whose page the cache does not have gets scale -1, which
+  // no row has: it is hidden.  (Every address that is worked out lies in the cache, whether it is used or not.)
+  auto ask = [&](const Piece& p, int tile) {
+#pragma unroll
+    for (int u = 0; u < TPW; ++u) {
+      if (tile + u < p.end_tile) {
+        const unsigned to = fill + u * Shape::TILE;
+        const int j0 = real_tile(p, tile + u) << 4;
+        if constexpr (FAST) {
+          const bool ok = (unsigned)ahead[u] < (unsigned)a.num_pages;
+          const int in_page = a.ps_shift >= 0 ? j0 & (a.ps - 1) : j0 % a.ps;
+          const int row = ok ? ahead[u] * a.page_rows + in_page : 0;      // rows of codes from the head's first one on: fewer than 2^31 in all
+          const int8_t *kp = p.k_lane + (long long)row * HDP, *vp = p.v_lane + (long long)row * HDP;
+#pragma unroll
+          for (int i = 0; i < HDP / 32; ++i) {
+            copy16(Q8Place<HDP>::copy(to + c_place, i), kp + i * 512);
+            copy16(Q8Place<HDP>::copy(to + c_place, i) + 16 * HDP, vp + i * 512);
+          }
+          const unsigned s_to = to + 32 * HDP + lane * 4;
+          if (ok) copy4(s_to, p.s_lane + row);
+          else asm volatile("st.shared.f32 [%0], %1;" ::"r"(s_to), "f"(-1.f) : "memory");
+        } else {
+#pragma unroll
+          for (int i = 0; i < HDP / 32; ++i) {
+            const int row = (lane + 32 * i) / (HDP / 16), byte = (lane + 32 * i) % (HDP / 16) * 16, j = j0 + row;
+            const int jt = min(j, a.max_blocks * a.ps - 1), page = p.bt[jt / a.ps];
+            const bool ok = j == jt && page >= 0 && page < a.num_pages;
+            const long long base = (ok ? (long long)page * a.page_rows + j % a.ps : 0) + p.hk * a.ps;
+            const int place = q8_place<HDP>(row, byte);
+            copy16(to + place, a.kc + base * hd + (byte < hd ? byte : 0), ok && byte < hd);
+            copy16(to + 16 * HDP + place, a.vc + base * hd + (byte < hd ? byte : 0), ok && byte < hd);
+            if (byte == 0) {
+              const unsigned s_to = to + 32 * HDP + row * 4;
+              if (ok) {
+                copy4(s_to, a.ks + base);
+                copy4(s_to + 64, a.vs + base);
+              } else {
+                asm volatile("st.shared.f32 [%0], %1;\n\tst.shared.f32 [%0 + 64], %1;" ::"r"(s_to), "f"(-1.f) : "memory");
+              }
+            }
+          }
+        }
+      }
+    }
+    copies_close();
+    fill = fill + Shape::STAGE == ring_end ? ring : fill + Shape::STAGE;
+  };
+  auto ask_first = [&](const Piece& p) {      // all stages but one
+    const int tile = p.u0 * UNIT + warp * TPW;
+    if (FAST && tile < p.end_tile) find_pages(p, tile);
+    for (int s = 0; s < a.stages - 1; ++s) {
+      ask(p, tile + s * UNIT);
+      if (FAST && tile + (s + 1) * UNIT < p.end_tile) find_pages(p, tile + (s + 1) * UNIT);
+    }
+  };
+
+  Piece cur;
+  find_piece(cur);
+  ask_first(cur);
+  while (true) {
+    const int live = cur.it.n_rows * cur.n_h, n_h = cur.n_h;
+    const int n_h_inv = (65536 + n_h - 1) / n_h;
+    auto row_in = [&](int m) { return m * n_h_inv >> 16; };      // m / n_h, exact for m and n_h up to 32
     // queries as three signed bytes a number, a warp to a query
-    for (int m = warp; m < NQ; m += Q8_WARPS) {
+    for (int m = warp; m < live; m += Q8_WARPS) {
       float x[HDP / 32];
       unsigned top = 0;
-      const TT* src = static_cast<const TT*>(a.q) + (size_t)(it.row0 + m / n_h) * a.ld + (h0 + m % n_h) * hd;
+      const TT* src = static_cast<const TT*>(a.q) + (size_t)(cur.it.row0 + row_in(m)) * a.ld + (cur.h0 + m - row_in(m) * n_h) * hd;
 #pragma unroll
       for (int i = 0; i < HDP / 32; ++i) {
-        x[i] = m < live && i * 32 + lane < hd ? to_f32(src[i * 32 + lane]) : 0.f;
+        x[i] = i * 32 + lane < hd ? to_f32(src[i * 32 + lane]) : 0.f;
         top = max(top, q8_bits(x[i]));
       }
 #pragma unroll
@@ -254,33 +455,26 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
       for (int i = 0; i < HDP / 32; ++i) {
         const int v = top < 0x7f800000u ? __float2int_rn(x[i] * f) : 0;
         const int lo = (int)(int8_t)v, v1 = (v - lo) >> 8, mid = (int)(int8_t)v1;
-        int8_t* dst = sm_q + m * LDQ + i * 32 + lane;
+        int8_t* dst = sm_q + m * LDQ + (lane >> 2 & 3) * (HDP / 4) + i * 8 + (lane >> 4) * 4 + (lane & 3);      // number d = 32 i + 16 h + 4 t + byte: what lane t needs lies together
         dst[0] = (int8_t)((v1 - mid) >> 8);
-        dst[NQ * LDQ] = (int8_t)mid;
-        dst[2 * NQ * LDQ] = (int8_t)lo;
+        dst[cols * LDQ] = (int8_t)mid;
+        dst[2 * cols * LDQ] = (int8_t)lo;
       }
       if (lane == 0) sm_f[m] = top < 0x7f800000u ? __uint_as_float((unsigned)(254 - up) << 23) : __uint_as_float(0x7fc00000u);
     }
     __syncthreads();
-    // ... as B fragments: column g of each n-tile; the contraction's order is that of the keys' pieces
-    auto q_words = [&](int digit, int nt, int c, unsigned (&w)[W]) {
-      const int8_t* p = sm_q + (digit * NQ + nt * 8 + g) * LDQ + (c * 16 + t * 4) * W;
-      if constexpr (W == 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p);
-        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-      } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        w[0] = v.x; w[1] = v.y;
-      }
-    };
-    unsigned qf[Q_IN_REGS ? 3 : 1][Q_IN_REGS ? NT : 1][Q_IN_REGS ? PIECES : 1][W];
+    // ... as B fragments: column g of each n-tile (a dead column repeats a live one)
+    constexpr int QW = 2 * STEPS < 4 ? 2 * STEPS : 4;      // words of a load
+    const unsigned q_at = (unsigned)__cvta_generic_to_shared(sm_q) + t * (HDP / 4);
+    auto q_words = [&](int digit, int nt, int x, unsigned* w) { read_words<QW>(w, q_at + (digit * cols + min(nt * 8 + g, live - 1)) * LDQ + x * 8); };
+    unsigned qf[Q_IN_REGS ? 3 : 1][Q_IN_REGS ? NT : 1][Q_IN_REGS ? 2 * STEPS : 1];
     if constexpr (Q_IN_REGS) {
 #pragma unroll
       for (int digit = 0; digit < 3; ++digit)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < PIECES; ++c) q_words(digit, nt, c, qf[digit][nt][c]);
+          for (int x = 0; x < STEPS; x += QW / 2) q_words(digit, nt, x, &qf[digit][nt][2 * x]);
     }
     // this lane's columns 2t and 2t + 1 of each n-tile: position, first key seen, factor of the score
     int qp[NT][2], qs[NT][2], qk[NT][2];
@@ -291,12 +485,12 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int m = min(nt * 8 + 2 * t + e, live - 1);
-        const float back = sm_f[nt * 8 + 2 * t + e] * a.scale;
-        qp[nt][e] = it.pos0 + max(m, 0) / n_h;
+        const float back = sm_f[m] * a.scale;
+        qp[nt][e] = cur.it.pos0 + row_in(m);
         qs[nt][e] = first_seen(qp[nt][e], a.window);
         qx[nt][e] = back * LOG2E;
         if constexpr (EXT) {
-          const int h = h0 + max(m, 0) % n_h;
+          const int h = cur.h0 + m - row_in(m) * n_h;
           qk[nt][e] = kept_end(qp[nt][e], a.window, a.keep);
           qx[nt][e] = back;
           if (a.temp_every > 0) qx[nt][e] *= 1.0f + a.temp_coef * logf((float)((qp[nt][e] + 1) / a.temp_every + 1));
@@ -304,257 +498,158 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
           qrate[nt][e] = a.rates ? a.rates + h : nullptr;
         }
       }
-    const int whole_from = first_seen(last, a.window), whole_to = it.pos0;      // keys that every row sees
+    const int whole_from = first_seen(cur.it.pos0 + cur.it.n_rows - 1, a.window), whole_to = cur.it.pos0;      // keys that every row sees
 
-    float o[NT][KS][4], m_run[NT][2], l_run[NT][2];
+    float o[NT][KS][4], m_run[NT][2], l_run[NT][2], ref[NT][2];      // ref: the running maximum, 0 while there is none
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < KS; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
       m_run[nt][0] = m_run[nt][1] = -INFINITY;
-      l_run[nt][0] = l_run[nt][1] = 0.f;
+      l_run[nt][0] = l_run[nt][1] = ref[nt][0] = ref[nt][1] = 0.f;
     }
 
-    unsigned kw[TPW][2][PIECES * W], vw[TPW][4][VW];
-    float ksc[TPW][2], vsc[TPW][2];
-    long long base[TPW];                     // FAST: the row of codes that a loaded tile begins with
-    int ahead[TPW];                          // FAST: the pages of the tiles to be loaded next, as the table names them
-    unsigned held = 0;                       // two bits a tile: this lane's keys g and g + 8 lie in a page of the cache
-    auto real_tile = [&](int n) { return n < span.nk ? n : n + span.skipped; };
-    auto find_pages = [&](int tile) {
-#pragma unroll
-      for (int u = 0; u < TPW; ++u) {
-        const int j0 = real_tile(min(tile + u, end_tile - 1)) << 4;
-        ahead[u] = bt[a.ps_shift >= 0 ? j0 >> a.ps_shift : j0 / a.ps];
+    for (int tile = cur.u0 * UNIT + warp * TPW; tile < cur.end_tile; tile += UNIT) {
+      // the oldest stage has arrived, and every lane is done with the one before it, which is filled again
+      if (a.stages == 2) copies_wait<0>();
+      else copies_wait<1>();
+      __syncwarp();
+      {
+        const int next = tile + (a.stages - 1) * UNIT;
+        ask(cur, next);
+        if (FAST && next + UNIT < cur.end_tile) find_pages(cur, next + UNIT);
       }
-    };
-    // The row of codes of the key at j.  Where the table names no page of the cache that is the head's first row of page 0, and `ok` is
-    // false: every address that is worked out here lies in the cache, whether it is used or not.
-    auto row_of = [&](int j, bool& ok) -> long long {
-      const int at = min(j, a.max_blocks * a.ps - 1), page = bt[at / a.ps];
-      ok = j == at && page >= 0 && page < a.num_pages;
-      return ok ? ((long long)page * a.n_kv_head + hk) * a.ps + j % a.ps : (long long)hk * a.ps;
-    };
-    auto load_keys = [&](int tile) {
-      held = 0;
+      const unsigned stage = use;
+      use = use + Shape::STAGE == ring_end ? ring : use + Shape::STAGE;
+      float s[TPW][NT][4], vx[TPW][2];
+      bool whole = true;       // every row sees every key of the warp's tiles
+      bool hidden = false;
 #pragma unroll
       for (int u = 0; u < TPW; ++u) {
-        if (tile + u >= end_tile) continue;
-        const int j0 = real_tile(tile + u) << 4;
-        if constexpr (FAST) {
-          const bool ok = ahead[u] >= 0 && ahead[u] < a.num_pages;
-          const int in_page = a.ps_shift >= 0 ? j0 & (a.ps - 1) : j0 % a.ps;
-          base[u] = ok ? ((long long)ahead[u] * a.n_kv_head + hk) * a.ps + in_page : (long long)hk * a.ps;
-          held |= ok ? 3u << (2 * u) : 0u;
-          const int8_t* p = a.kc + base[u] * HDP + (g * HDP + t * 4 * W);
+        if (tile + u >= cur.end_tile) {
+          whole = false;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int c = 0; c < PIECES; ++c) load_words<W>(&kw[u][i][c * W], p + i * 8 * HDP + c * 16 * W);
-          const float *ps = a.ks + base[u] + g, *vs = a.vs + base[u] + g;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            ksc[u][i] = load_float(ps + 8 * i);
-            vsc[u][i] = load_float(vs + 8 * i);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            bool ok;
-            const long long row = row_of(j0 + g + 8 * i, ok);
-            if (ok) held |= 1u << (2 * u + i);
-            const int8_t* p = a.kc + row * hd;
-#pragma unroll
-            for (int c = 0; c < PIECES; ++c) {
-              const int d0 = c * 16 * W + t * 4 * W;
-              load_words<W>(&kw[u][i][c * W], p + (d0 < hd ? d0 : 0));
-              if (d0 >= hd) {
-#pragma unroll
-                for (int w = 0; w < W; ++w) kw[u][i][c * W + w] = 0;
-              }
-            }
-            ksc[u][i] = load_float(a.ks + row);
-            vsc[u][i] = load_float(a.vs + row);
-          }
+          for (int nt = 0; nt < NT; ++nt) s[u][nt][0] = s[u][nt][1] = s[u][nt][2] = s[u][nt][3] = -INFINITY;
+          continue;
         }
-      }
-    };
-    auto load_values = [&](int tile) {      // after load_keys(tile), before the next load_keys
+        const unsigned st = stage + u * Shape::TILE, sc = st + 32 * HDP + g * 4;
+        const int j0 = real_tile(cur, tile + u) << 4;
+        unsigned kw[STEPS][4];
 #pragma unroll
-      for (int u = 0; u < TPW; ++u) {
-        if (tile + u >= end_tile) continue;
-        constexpr int PW = VW < 4 ? VW : 4;      // words of a load
-        if constexpr (FAST) {
-          const int8_t* p = a.vc + base[u] * HDP + (2 * t * HDP + g * 4 * VW);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int w0 = 0; w0 < VW; w0 += PW) load_words<PW>(&vw[u][i][w0], p + ((i & 1) + 8 * (i >> 1)) * HDP + 4 * w0);
-        } else {
-          const int j0 = real_tile(tile + u) << 4;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            bool ok;
-            const int8_t* p = a.vc + row_of(j0 + 2 * t + (i & 1) + 8 * (i >> 1), ok) * hd;
-#pragma unroll
-            for (int w0 = 0; w0 < VW; w0 += PW) {
-              const int d0 = (g * VW + w0) * 4;
-              load_words<PW>(&vw[u][i][w0], p + (d0 < hd ? d0 : 0));
-              if (d0 >= hd) {
-#pragma unroll
-                for (int w = 0; w < PW; ++w) vw[u][i][w0 + w] = 0;
-              }
-            }
-          }
-        }
-      }
-    };
-    // tiles behind the last are not loaded: their products are masked, but have to be of something
-#pragma unroll
-    for (int u = 0; u < TPW; ++u) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        ksc[u][i] = vsc[u][i] = 0.f;
-#pragma unroll
-        for (int w = 0; w < PIECES * W; ++w) kw[u][i][w] = 0;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int w = 0; w < VW; ++w) vw[u][i][w] = 0;
-    }
-
-    int tile = u0 * UNIT + warp * TPW;
-    if (tile < end_tile) {
-      if constexpr (FAST) find_pages(tile);
-      load_keys(tile);
-      load_values(tile);
-      if constexpr (FAST) find_pages(tile + UNIT);
-    }
-    // A round: the scores are taken from the keys, the keys of the next round are asked for, the maxima, sums and products with the
-    // values follow, and the next values are asked for: a warp has loads on their way all the time.
-    for (; tile < end_tile; tile += UNIT) {
-      float s[TPW][NT][4];
-#pragma unroll
-      for (int u = 0; u < TPW; ++u) {
+        for (int x = 0; x < STEPS; ++x) read_keys(kw[x], Q8Place<HDP>::key(st + k_place, x));
+        const float kx[2] = {read_float(sc), read_float(sc + 32)};
+        vx[u][0] = read_float(sc + 64);
+        vx[u][1] = read_float(sc + 96);
+        whole = whole && j0 >= whole_from && j0 + 15 <= whole_to;
+        hidden = hidden || fminf(kx[0], kx[1]) < 0.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          int sh[4] = {0, 0, 0, 0}, sd[4] = {0, 0, 0, 0}, sl[4] = {0, 0, 0, 0};
+          int sh[4], sd[4], sl[4];
 #pragma unroll
-          for (int c = 0; c < PIECES; ++c) {
-            unsigned q0[W], q1[W], q2[W];
+          for (int x0 = 0; x0 < STEPS; x0 += QW / 2) {
+            unsigned q0[QW], q1[QW], q2[QW];
             if constexpr (Q_IN_REGS) {
 #pragma unroll
-              for (int w = 0; w < W; ++w) {
-                q0[w] = qf[0][nt][c][w];
-                q1[w] = qf[1][nt][c][w];
-                q2[w] = qf[2][nt][c][w];
+              for (int w = 0; w < QW; ++w) {
+                q0[w] = qf[0][nt][2 * x0 + w];
+                q1[w] = qf[1][nt][2 * x0 + w];
+                q2[w] = qf[2][nt][2 * x0 + w];
               }
             } else {
-              q_words(0, nt, c, q0);
-              q_words(1, nt, c, q1);
-              q_words(2, nt, c, q2);
+              q_words(0, nt, x0, q0);
+              q_words(1, nt, x0, q1);
+              q_words(2, nt, x0, q2);
             }
 #pragma unroll
-            for (int w = 0; w < W; w += 2) {
-              const unsigned A[4] = {kw[u][0][c * W + w], kw[u][1][c * W + w], kw[u][0][c * W + w + 1], kw[u][1][c * W + w + 1]};
-              mma_16832_s8(sh, A, q0[w], q0[w + 1]);
-              mma_16832_s8(sd, A, q1[w], q1[w + 1]);
-              mma_16832_s8(sl, A, q2[w], q2[w + 1]);
+            for (int w = 0; w < QW; w += 2) {
+              const int x = x0 + w / 2;
+              if (x == 0) {
+                mma_16832_s8_first(sh, kw[x], q0[w], q0[w + 1]);
+                mma_16832_s8_first(sd, kw[x], q1[w], q1[w + 1]);
+                mma_16832_s8_first(sl, kw[x], q2[w], q2[w + 1]);
+              } else {
+                mma_16832_s8(sh, kw[x], q0[w], q0[w + 1]);
+                mma_16832_s8(sd, kw[x], q1[w], q1[w + 1]);
+                mma_16832_s8(sl, kw[x], q2[w], q2[w + 1]);
+              }
             }
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[u][nt][e] = fmaf((float)sh[e], 65536.f, (float)(sd[e] * 256 + sl[e]));
-        }
-      }
-      float kx[TPW][2], vx[TPW][2];
-      const unsigned in_page = held;
-#pragma unroll
-      for (int u = 0; u < TPW; ++u)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          kx[u][i] = ksc[u][i];
-          vx[u][i] = vsc[u][i];
-        }
-      if (tile + UNIT < end_tile) {
-        load_keys(tile + UNIT);
-        if constexpr (FAST) find_pages(tile + 2 * UNIT);
-      }
-      // scores in the base-2 domain; -inf where the query does not see the key
-      bool whole = true;       // every row sees every key of the warp's tiles
-      float mx[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < TPW; ++u) {
-        const int j0 = real_tile(tile + u) << 4;
-        whole = whole && tile + u < end_tile && j0 >= whole_from && j0 + 15 <= whole_to;
-        if constexpr (FAST) whole = whole && ((in_page >> (2 * u)) & 3u) == 3u;      // the same in all lanes
-        else whole = whole && __all_sync(0xffffffffu, ((in_page >> (2 * u)) & 3u) == 3u);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          // scores in the base-2 domain
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int i = e >> 1, c = e & 1;
-            float v = s[u][nt][e] * (kx[u][i] * qx[nt][c]);
+            const int c = e & 1;
+            float v = fmaf((float)sh[e], 65536.f, (float)(sd[e] * 256 + sl[e])) * (kx[e >> 1] * qx[nt][c]);
             if constexpr (EXT) {
               v = capped_score(v, a.cap);
-              if (a.slopes) v -= distance_bias(qslope[nt][c], qrate[nt][c], (float)max(qp[nt][c] - (j0 + g + 8 * i), 0));
+              if (a.slopes) v -= distance_bias(qslope[nt][c], qrate[nt][c], (float)max(qp[nt][c] - (j0 + g + 8 * (e >> 1)), 0));
               v *= LOG2E;
             }
             s[u][nt][e] = v;
           }
-      }
-      if (!whole) {
-#pragma unroll
-        for (int u = 0; u < TPW; ++u) {
-          const int j0 = real_tile(tile + u) << 4;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int i = e >> 1, c = e & 1, j = j0 + g + 8 * i;
-              const bool ok = tile + u < end_tile && j <= qp[nt][c] && (j >= qs[nt][c] || (EXT && j < qk[nt][c])) && ((in_page >> (2 * u + i)) & 1u);
-              s[u][nt][e] = ok ? s[u][nt][e] : -INFINITY;
-            }
         }
       }
+      whole = whole && !__any_sync(0xffffffffu, hidden);
+      if (!whole) {             // -inf where the query does not see the key
 #pragma unroll
-      for (int u = 0; u < TPW; ++u)
+        for (int u = 0; u < TPW; ++u) {
+          if (tile + u >= cur.end_tile) continue;
+          const int j0 = real_tile(cur, tile + u) << 4;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int i = 0; i < 2; ++i) {
+            const int j = j0 + g + 8 * i;
+            const bool there = !(read_float(stage + u * Shape::TILE + 32 * HDP + (g + 8 * i) * 4) < 0.f);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const bool ok = there && j <= qp[nt][c] && (j >= qs[nt][c] || (EXT && j < qk[nt][c]));
+                s[u][nt][2 * i + c] = ok ? s[u][nt][2 * i + c] : -INFINITY;
+              }
+          }
+        }
+      }
+      float mx[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mx[nt][0] = mx[nt][1] = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < TPW; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e) mx[nt][e & 1] = fmaxf(mx[nt][e & 1], s[u][nt][e]);
+      }
       bool moved = false;
-      float corr[NT][2], ref[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) mx[nt][c] = fmaxf(mx[nt][c], __shfl_xor_sync(0xffffffffu, mx[nt][c], x));
-          const float m_new = fmaxf(m_run[nt][c], mx[nt][c]);
-          moved |= m_new != m_run[nt][c];
-          ref[nt][c] = m_new == -INFINITY ? 0.f : m_new;
-          corr[nt][c] = ex2(m_run[nt][c] - ref[nt][c]);
-          m_run[nt][c] = m_new;
+          moved |= mx[nt][c] > m_run[nt][c];
         }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          l_run[nt][0] *= corr[nt][0];
-          l_run[nt][1] *= corr[nt][1];
+          float corr[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float m_new = fmaxf(m_run[nt][c], mx[nt][c]);
+            ref[nt][c] = m_new == -INFINITY ? 0.f : m_new;
+            corr[c] = ex2(m_run[nt][c] - ref[nt][c]);
+            m_run[nt][c] = m_new;
+            l_run[nt][c] *= corr[c];
+          }
 #pragma unroll
           for (int j = 0; j < KS; ++j) {
-            o[nt][j][0] *= corr[nt][0];
-            o[nt][j][1] *= corr[nt][1];
-            o[nt][j][2] *= corr[nt][0];
-            o[nt][j][3] *= corr[nt][1];
+            o[nt][j][0] *= corr[0];
+            o[nt][j][1] *= corr[1];
+            o[nt][j][2] *= corr[0];
+            o[nt][j][3] *= corr[1];
           }
         }
       }
 #pragma unroll
       for (int u = 0; u < TPW; ++u) {
+        if (tile + u >= cur.end_tile) continue;
         unsigned pf[PARTS][NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -579,104 +674,126 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
             }
           }
         }
+        const unsigned v_at = stage + u * Shape::TILE + v_place;
 #pragma unroll
-        for (int j = 0; j < KS; ++j) {
-          const int w = j >> 1;
-          const unsigned lo = j & 1 ? 0x0602 : 0x0400, hi = j & 1 ? 0x0703 : 0x0501;
-          const unsigned A[4] = {q8_pair(__byte_perm(vw[u][0][w], vw[u][1][w], lo)), q8_pair(__byte_perm(vw[u][0][w], vw[u][1][w], hi)),
-                                 q8_pair(__byte_perm(vw[u][2][w], vw[u][3][w], lo)), q8_pair(__byte_perm(vw[u][2][w], vw[u][3][w], hi))};
+        for (int w0 = 0; w0 < VW; w0 += PW) {
+          unsigned vw[4][PW];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int i = 0; i < 4; ++i) read_words<PW>(vw[i], (i & 1 ? Q8Place<HDP>::odd(v_at ^ (w0 * 4)) : v_at ^ (w0 * 4)) + (i >> 1) * 8 * HDP);
 #pragma unroll
-            for (int p = PARTS - 1; p >= 0; --p) mma_16816(o[nt][j], A, pf[p][nt][0], pf[p][nt][1]);
+          for (int j = 0; j < 2 * PW; ++j) {
+            const int w = j >> 1;
+            const unsigned lo = j & 1 ? 0x0602 : 0x0400, hi = j & 1 ? 0x0703 : 0x0501;
+            const unsigned A[4] = {q8_pair(__byte_perm(vw[0][w], vw[1][w], lo), base), q8_pair(__byte_perm(vw[0][w], vw[1][w], hi), base),
+                                   q8_pair(__byte_perm(vw[2][w], vw[3][w], lo), base), q8_pair(__byte_perm(vw[2][w], vw[3][w], hi), base)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int p = PARTS - 1; p >= 0; --p) mma_16816(o[nt][2 * w0 + j], A, pf[p][nt][0], pf[p][nt][1]);
+          }
         }
       }
-      if (tile + UNIT < end_tile) load_values(tile + UNIT);
+    }
+    // what was asked for behind the piece's end is nothing; the next piece's first tiles are on their way while this one is finished
+    copies_wait<0>();
+    __syncwarp();
+    fill = use = ring;
+    const bool more = w_at < w_end;
+    const Piece done = cur;
+    if (more) {
+      find_piece(cur);
+      ask_first(cur);
     }
 
-    // the warps' results joined
+    // the warps' results joined, eight columns at a time
+    const bool alone = done.begins && done.ends;
+    float* mine = a.part + (size_t)(2 * blockIdx.x + done.begins) * NQ * (HDP + 2);
+    // entry i of a query's row in shared memory is [pair of dims j][lane g][2]: the dim
+    auto dim_of = [&](int i) { return ((i >> 1) & 7) * (HDP / 8) + (i >> 4) * 2 + (i & 1); };
+    const int jq = min(cols, 8);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      if (nt * 8 < live) {
+        if (nt > 0) __syncthreads();
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float l = l_run[nt][c];
+        for (int c = 0; c < 2; ++c) {
+          float l = l_run[nt][c];
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-        const int m = nt * 8 + 2 * t + c;
-        if (g == 0) {
-          sm_m[warp * NQ + m] = m_run[nt][c];
-          sm_l[warp * NQ + m] = l;
+          for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+          if (g == 0) {
+            sm_m[warp * 8 + 2 * t + c] = m_run[nt][c];
+            sm_l[warp * 8 + 2 * t + c] = l;
+          }
+          if (nt * 8 + 2 * t + c < live) {
+            float* dst = sm_acc + (size_t)(warp * jq + 2 * t + c) * LDS + g * 2;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) *reinterpret_cast<float2*>(dst + j * 16) = make_float2(o[nt][j][c], o[nt][j][2 + c]);
+          }
         }
-        if (m < live) {
-          float* dst = sm_acc + (size_t)(warp * NQ + m) * LDS + g * 2;      // [pair of dims j][lane g][2]
+        __syncthreads();
+        for (int x = tid; x < min(live - nt * 8, 8) * HDP; x += Q8_THREADS) {
+          const int mq = x / HDP, i = x % HDP, m = nt * 8 + mq, d = dim_of(i);
+          float mw[Q8_WARPS], M = -INFINITY, l = 0.f, v = 0.f;
 #pragma unroll
-          for (int j = 0; j < KS; ++j) *reinterpret_cast<float2*>(dst + j * 16) = make_float2(o[nt][j][c], o[nt][j][2 + c]);
-        }
-      }
-    __syncthreads();
-    const bool alone = u0 == 0 && u1 == units;
-    const long long item_at = (long long)hg * total + before[item];
-    const int b_first = (int)(item_at / per), b_last = (int)((item_at + units - 1) / per);
-    float* mine = a.part + (size_t)(2 * blockIdx.x + (u0 == 0)) * NQ * (HDP + 2);
-    for (int x = tid; x < live * HDP; x += Q8_THREADS) {
-      const int m = x / HDP, i = x % HDP, d = ((i >> 1) & 7) * (HDP / 8) + (i >> 4) * 2 + (i & 1);
-      float mw[Q8_WARPS], M = -INFINITY, l = 0.f, v = 0.f;
+          for (int w = 0; w < Q8_WARPS; ++w) {
+            mw[w] = sm_m[w * 8 + mq];
+            M = fmaxf(M, mw[w]);
+          }
 #pragma unroll
-      for (int w = 0; w < Q8_WARPS; ++w) {
-        mw[w] = sm_m[w * NQ + m];
-        M = fmaxf(M, mw[w]);
-      }
-#pragma unroll
-      for (int w = 0; w < Q8_WARPS; ++w) {
-        const float f = mw[w] == -INFINITY && M != -INFINITY ? 0.f : ex2(mw[w] - (M == -INFINITY ? 0.f : M));
-        v = fmaf(f, sm_acc[(size_t)(w * NQ + m) * LDS + i], v);
-        l = fmaf(f, sm_l[w * NQ + m], l);
-      }
-      if (alone) {
-        const int h = h0 + m % n_h;
-        float keep1 = 1.f;
-        if (a.sinks) {
-          const float sk = a.sinks[h] * LOG2E, mm = fmaxf(M, sk);
-          keep1 = ex2(M - mm);
-          l = fmaf(l, keep1, ex2(sk - mm));
-        }
-        if (d < hd) from_f32(static_cast<TT*>(a.out)[(size_t)(it.row0 + m / n_h) * a.out_ld + h * hd + d], l == 0.f ? 0.f : v * keep1 / l);
-      } else {
-        float* p = mine + m * (HDP + 2);
-        p[2 + i] = v;
-        if (i == 0) {
-          p[0] = M;
-          p[1] = l;
+          for (int w = 0; w < Q8_WARPS; ++w) {
+            const float f = mw[w] == -INFINITY && M != -INFINITY ? 0.f : ex2(mw[w] - (M == -INFINITY ? 0.f : M));
+            v = fmaf(f, sm_acc[(size_t)(w * jq + mq) * LDS + i], v);
+            l = fmaf(f, sm_l[w * 8 + mq], l);
+          }
+          if (alone) {
+            const int h = done.h0 + m - row_in(m) * n_h;
+            float keep1 = 1.f;
+            if (a.sinks) {
+              const float sk = a.sinks[h] * LOG2E, mm = fmaxf(M, sk);
+              keep1 = ex2(M - mm);
+              l = fmaf(l, keep1, ex2(sk - mm));
+            }
+            if (d < hd) from_f32(static_cast<TT*>(a.out)[(size_t)(done.it.row0 + row_in(m)) * a.out_ld + h * hd + d], l == 0.f ? 0.f : v * keep1 / l);
+          } else {
+            float* p = mine + m * (HDP + 2);
+            p[2 + i] = v;
+            if (i == 0) {
+              p[0] = M;
+              p[1] = l;
+            }
+          }
         }
       }
     }
     if (!alone) {
+      // the cuts that were left inside the item; the piece behind cut c is block c's, the first piece that of the block before
+      const long long begin = (long long)done.hg * total + before[done.item], end = begin + before[done.item + 1] - before[done.item];
+      const int b_first = (int)((begin + slack) / per), n_pieces = (int)((end - slack - 1) / per) - b_first + 1;
       __threadfence();
       __syncthreads();
-      unsigned* counter = a.counters + (size_t)item * n_hg + hg;
-      if (tid == 0) sm_i[0] = atomicAdd(counter, 1u) == (unsigned)(b_last - b_first);
+      unsigned* counter = a.counters + (size_t)done.item * n_hg + done.hg;
+      if (tid == 0) sm_i[0] = atomicAdd(counter, 1u) == (unsigned)(n_pieces - 1);
       __syncthreads();
       if (sm_i[0]) {
         __threadfence();
-        const int n_pieces = b_last - b_first + 1;
         auto piece = [&](int b) { return a.part + (size_t)(2 * (b_first + b) + (b == 0)) * NQ * (HDP + 2); };
         // every query's maximum and sum over the pieces first
         for (int m = warp; m < live; m += Q8_WARPS) {
           float M = -INFINITY, l = 0.f;
           for (int b = lane; b < n_pieces; b += 32) M = fmaxf(M, load_float(piece(b) + m * (HDP + 2)));
           M = warp_max(M);
-          const float sk = a.sinks ? a.sinks[h0 + m % n_h] * LOG2E : -INFINITY, mm = fmaxf(M, sk), r = mm == -INFINITY ? 0.f : mm;
+          const float sk = a.sinks ? a.sinks[done.h0 + m - row_in(m) * n_h] * LOG2E : -INFINITY, mm = fmaxf(M, sk), r = mm == -INFINITY ? 0.f : mm;
           for (int b = lane; b < n_pieces; b += 32) l = fmaf(ex2(load_float(piece(b) + m * (HDP + 2)) - r), load_float(piece(b) + m * (HDP + 2) + 1), l);
           l = warp_sum(l) + (a.sinks ? ex2(sk - r) : 0.f);
           if (lane == 0) {
             sm_w[m] = r;
-            sm_w[NQ + m] = l;
+            sm_w[32 + m] = l;
           }
         }
         __syncthreads();
         for (int x = tid; x < live * HDP; x += Q8_THREADS) {
-          const int m = x / HDP, i = x % HDP, d = ((i >> 1) & 7) * (HDP / 8) + (i >> 4) * 2 + (i & 1);
-          const float r = sm_w[m], l = sm_w[NQ + m];
+          const int m = x / HDP, i = x % HDP, d = dim_of(i);
+          const float r = sm_w[m], l = sm_w[32 + m];
           float v = 0.f;
           for (int b0 = 0; b0 < n_pieces; b0 += 8) {      // eight in flight
             float pm[8], pv[8];
@@ -689,30 +806,37 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
 #pragma unroll
             for (int b = 0; b < 8; ++b) v = b0 + b < n_pieces ? fmaf(ex2(pm[b] - r), pv[b], v) : v;
           }
-          const int h = h0 + m % n_h;
-          if (d < hd) from_f32(static_cast<TT*>(a.out)[(size_t)(it.row0 + m / n_h) * a.out_ld + h * hd + d], l == 0.f ? 0.f : v / l);
+          const int h = done.h0 + m - row_in(m) * n_h;
+          if (d < hd) from_f32(static_cast<TT*>(a.out)[(size_t)(done.it.row0 + row_in(m)) * a.out_ld + h * hd + d], l == 0.f ? 0.f : v / l);
         }
         if (tid == 0) *counter = 0;
       }
     }
-    __syncthreads();
-    w_at += u1 - u0;
+    if (!more) break;
+    __syncthreads();      // the next piece's queries and sums go where this one's were
   }
 }
 
 // How a launch is laid out.
 struct Q8Plan {
-  int hdp, nt, heads_per, head_blocks, rows_per, tiles_per_seg;
+  int hdp, nt, heads_per, head_blocks, rows_per, tiles_per_seg, stages, smem;
   long long items, blocks, floats, counters;
 };
 
 template <int HDP, int NT, int PARTS, bool EXT, bool FAST>
 int q8_launch(const Q8Args& a, const Q8Plan& p, cudaStream_t st) {
   auto kern = attention_q8_kernel<HDP, NT, PARTS, EXT, FAST>;
-  const size_t smem = Q8Shape<HDP, NT, PARTS>::smem(a.n_items);
-  const cudaError_t e = allow_smem(kern, smem);
+  // the kernel's limit on shared memory is set once a device (a call takes the host some 10 us)
+  static std::atomic<unsigned long long> set{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(kern, dim3((unsigned)p.blocks), dim3(Q8_THREADS), smem, st, a);
+  if (dev < 0 || dev >= 64 || !(set.load(std::memory_order_acquire) >> dev & 1)) {
+    e = allow_smem(kern, 200 * 1024);
+    if (e != cudaSuccess) return (int)e;
+    if (dev >= 0 && dev < 64) set.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  return (int)launch_pdl(kern, dim3((unsigned)p.blocks), dim3(Q8_THREADS), p.smem, st, a);
 }
 template <int HDP, int NT, int PARTS>
 int q8_launch2(const Q8Args& a, const Q8Plan& p, bool ext, cudaStream_t st) {
@@ -734,6 +858,5 @@ int q8_run(const Q8Args& a, const Q8Plan& p, bool ext, int f32, cudaStream_t st)
     if (p.nt == 4) return q8_launch2<HDP, 4, 1>(a, p, ext, st);
   return CBIS_ERR_BAD_SIZE;
 }
-
 
 }  // namespace cbis
