@@ -20,7 +20,7 @@ int columns8(int hdp, int f32, long long queries) {
   const int nt = queries <= 8 ? 1 : (queries <= 16 ? 2 : 4);
   return nt < most ? nt : most;
 }
-int blocks_per_sm(int hdp, int nt, int f32) { return nt == 1 && hdp < 256 ? (f32 ? 3 : 4) : 2; }      // as Q8Shape::BLOCKS
+int blocks_per_sm(int hdp, int nt, int f32) { return nt == 1 && hdp < 256 ? (f32 || hdp == 128 ? 3 : 4) : 2; }      // as Q8Shape::BLOCKS
 
 // rows_of_seg 0: decoding, `n` rows; else `n` requests of at most so many rows.
 Q8Plan q8_plan(int n, int rows_of_seg, int n_head, int n_kv_head, int hd, int f32, int max_context) {
@@ -35,18 +35,26 @@ Q8Plan q8_plan(int n, int rows_of_seg, int n_head, int n_kv_head, int hd, int f3
   p.tiles_per_seg = (int)((rows + p.rows_per - 1) / p.rows_per);
   p.items = (long long)n * p.tiles_per_seg;
   if (p.items > Q8_MAX_ITEMS) return p;
-  // three stages a warp where that many blocks still fit on an SM, else two
-  const int stage = (p.hdp >= 128 ? 1 : 128 / p.hdp) * (32 * p.hdp + 128), ldq = p.hdp >= 128 ? p.hdp + 16 : p.hdp;
-  int fit_blocks = blocks_per_sm(p.hdp, p.nt, f32);
-  for (p.stages = 3;; p.stages = 2) {
-    p.smem = q8_smem(stage, p.hdp + 8, ldq, p.stages, p.rows_per * p.heads_per, (int)p.items).bytes;
-    if (fit_blocks * (p.smem + 1024) <= 228 * 1024 || p.stages == 2) break;
+  // as many blocks on an SM as registers allow, if need be with two stages a warp instead of three, and with fewer columns joined at a time
+  const int tpw = p.hdp >= 256 ? 1 : (p.hdp == 128 ? (p.nt == 1 ? 2 : 1) : 128 / p.hdp);
+  const int stage = tpw * (32 * p.hdp + 128), ldq = p.hdp >= 128 ? p.hdp + 16 : p.hdp, cols = p.rows_per * p.heads_per;
+  for (int fit_blocks = blocks_per_sm(p.hdp, p.nt, f32);; --fit_blocks) {
+    bool fits = false;
+    for (int least = cols < 2 || p.nt > 1 ? 8 : 2, x = 0; x < 4 && !fits; ++x) {
+      p.stages = x < 2 ? 3 : 2;
+      p.join_cols = x % 2 == 0 ? 8 : least;
+      if (p.join_cols > cols) p.join_cols = cols;
+      p.smem = q8_smem(stage, p.hdp + 8, ldq, p.stages, cols, p.join_cols, (int)p.items).bytes;
+      fits = fit_blocks * (p.smem + 1024) <= 228 * 1024;
+    }
+    if (fits || fit_blocks == 1) {
+      p.blocks = 148LL * fit_blocks;
+      break;
+    }
   }
-  while (fit_blocks > 1 && fit_blocks * (p.smem + 1024) > 228 * 1024) --fit_blocks;
-  const long long unit = 64 * (p.hdp >= 128 ? 1 : 128 / p.hdp), pairs = p.items * n_kv_head * p.head_blocks;
-  const long long units = pairs * ((max_context + unit - 1) / unit + 1), slots = 148LL * fit_blocks;
-  p.blocks = units < slots ? units : slots;
-  p.floats = p.blocks * 2 * 8 * p.nt * (p.hdp + 2);
+  const long long pairs = p.items * n_kv_head * p.head_blocks, most = pairs * (max_context / (128 * tpw) + 2);      // no more blocks than there can be pieces
+  if (most < p.blocks) p.blocks = most;
+  p.floats = p.blocks * 2 * 8 * p.nt * (p.hdp + 4);
   p.counters = pairs;
   return p;
 }
@@ -86,7 +94,8 @@ CBIS_EXPORT int cbis_attention_q8(const void* q, int ld, int k_off, int v_off, v
   const int f32 = dtype == CBIS_F32, align = f32 ? 4 : 8;
   if (ld % align || (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15)) return CBIS_ERR_ALIGNMENT;
   const Q8Plan p = q8_plan(n, rows_of_seg, n_head, n_kv_head, hd, f32, max_context);
-  if (p.items > Q8_MAX_ITEMS || p.items * ((long long)max_blocks * ps / 64 + 3) > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;      // the units are counted in 32 bits
+  if (p.items > Q8_MAX_ITEMS || p.items * ((long long)max_blocks * ps / 16 + 8) > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;      // the tiles are counted in 32 bits
+  if ((uintptr_t)part & 15) return CBIS_ERR_ALIGNMENT;
   if (part_floats < p.floats || n_counters < p.counters || (k_off >= 0 && slot_mapping == nullptr)) return CBIS_ERR_BAD_SIZE;
   Q8Args a = {};
   a.q = q; a.out = out; a.kc = (int8_t*)kc; a.vc = (int8_t*)vc; a.ks = (float*)ks; a.vs = (float*)vs;
@@ -96,7 +105,7 @@ CBIS_EXPORT int cbis_attention_q8(const void* q, int ld, int k_off, int v_off, v
   a.n_rows = n_rows; a.ld = ld; a.out_ld = out_ld; a.k_off = k_off; a.v_off = v_off; a.max_blocks = max_blocks; a.num_pages = num_pages; a.n_seqs = n_seqs;
   a.seg0 = seg0; a.n_items = (int)p.items; a.tiles_per_seg = p.tiles_per_seg; a.n_head = n_head; a.n_kv_head = n_kv_head;
   a.heads_per = p.heads_per; a.head_blocks = p.head_blocks; a.rows_per = p.rows_per;
-  a.stages = p.stages; a.page_rows = n_kv_head * ps; a.hd = hd; a.ps = ps; a.ps_shift = -1;
+  a.stages = p.stages; a.join_cols = p.join_cols; a.page_rows = n_kv_head * ps; a.hd = hd; a.ps = ps; a.ps_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (ps == 1 << i) a.ps_shift = i;
   a.window = window; a.keep = keep; a.temp_every = temp_every; a.scale = scale; a.cap = cap; a.temp_coef = temp_coef;

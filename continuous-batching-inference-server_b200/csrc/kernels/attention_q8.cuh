@@ -16,10 +16,9 @@
 // 16-byte asynchronous copies and reads without two lanes on one bank (q8_place): what is on its way holds no registers, so four
 // blocks fit on an SM, and a block asks for the first tiles of its next piece before it finishes the one in hand.
 //
-// The keys of all (row, head) pairs are one row of units (16 KB of codes, and one more for what a pair costs beside them), which is cut
+// The tiles of 16 keys of all (row, head) pairs, and for every pair a few more for what it costs beside them, are one row that is cut
 // evenly over the blocks: every block works out its part from the positions on the device.  A cut that would leave a short end of a
-// pair is moved to the pair's end: a pair that lies in several blocks is merged by the last one to finish it, which takes as long as
-// some three units.
+// pair is moved to the pair's end: a pair that lies in several blocks is merged by the last one to finish it.
 #pragma once
 #include "cache_q8.cuh"
 #include "mma_sync.cuh"
@@ -30,7 +29,7 @@
 namespace cbis {
 
 constexpr int Q8_WARPS = 4, Q8_THREADS = Q8_WARPS * 32, Q8_MAX_ITEMS = 4096;
-constexpr int Q8_PAIR = 1, Q8_MERGE = 3;      // what a pair and a merge cost, in units
+constexpr int Q8_PAIR = 6;      // what a pair costs beside its keys, in tiles
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Q8Args {
@@ -43,7 +42,7 @@ struct Q8Args {
   unsigned* counters;
   const float *sinks, *slopes, *rates;
   int n_rows, ld, out_ld, k_off, v_off, max_blocks, num_pages, n_seqs, seg0, n_items, tiles_per_seg, n_head, n_kv_head, heads_per, head_blocks, rows_per;
-  int stages, page_rows, hd, ps, ps_shift, window, keep, temp_every;      // ps_shift: log2 of the page size, -1 where that is no whole number
+  int stages, join_cols, page_rows, hd, ps, ps_shift, window, keep, temp_every;      // ps_shift: log2 of the page size, -1 where that is no whole number
   float scale, cap, temp_coef;
 };
 
@@ -176,26 +175,25 @@ struct Q8Place {
 // 32-bit rows); EXT: kept first keys, a cap, a distance bias, a query temperature; FAST: the width is HDP and pages are a multiple of 16 keys.
 template <int HDP, int NT, int PARTS>
 struct Q8Shape {
-  static constexpr int TPW = HDP >= 128 ? 1 : 128 / HDP;        // tiles a warp takes through one update of its maxima and sums: a stage of its ring
-  static constexpr int UNIT = Q8_WARPS * TPW;                   // tiles of a unit
+  static constexpr int TPW = HDP >= 256 ? 1 : (HDP == 128 ? (NT == 1 ? 2 : 1) : 128 / HDP);        // tiles a warp takes through one update of its maxima and sums: a stage of its ring
+  static constexpr int UNIT = Q8_WARPS * TPW;                   // tiles that the warps take in a round
   static constexpr int NQ = 8 * NT;
   static constexpr int LDS = HDP + 8;                           // floats of a query's sums in shared memory
   static constexpr int LDQ = HDP >= 128 ? HDP + 16 : HDP;       // bytes of a query's row in shared memory: no two lanes of a load on one bank
   static constexpr int TILE = 32 * HDP + 128;                   // bytes of 16 keys: codes of keys, of values, their scales
   static constexpr int STAGE = TPW * TILE;
-  static constexpr int BLOCKS = NT == 1 && HDP < 256 ? (PARTS == 1 ? 4 : 3) : 2;      // per SM, as far as registers go
+  static constexpr int BLOCKS = NT == 1 && HDP < 256 ? (PARTS == 1 && HDP < 128 ? 4 : 3) : 2;      // per SM, as far as registers go
 };
-// Shared memory of a block (in this order): the warps' rings; sums, maxima of up to 8 columns from four warps; the queries' bytes; the
+// Shared memory of a block (in this order): the warps' rings; sums of jq columns from four warps, maxima of 8; the queries' bytes; the
 // columns' powers of two, merged maxima and sums; a few integers; the items.
 struct Q8Smem {
   int ring, join, stats, queries, columns, ints, items, bytes;
 };
-__host__ __device__ inline Q8Smem q8_smem(int stage, int lds, int ldq, int stages, int live, int n_items) {
+__host__ __device__ inline Q8Smem q8_smem(int stage, int lds, int ldq, int stages, int live, int jq, int n_items) {
   Q8Smem s;
-  const int jq = live < 8 ? live : 8;
   s.ring = 0;
   s.join = Q8_WARPS * stages * stage;
-  s.stats = s.join + Q8_WARPS * jq * lds * 4;
+  s.stats = s.join + (Q8_WARPS * jq * lds * 4 > 2048 ? Q8_WARPS * jq * lds * 4 : 2048);      // (2 KB: the groups' sums of a merge)
   s.queries = s.stats + Q8_WARPS * 8 * 2 * 4;
   s.columns = s.queries + 3 * live * ldq;
   s.ints = s.columns + 3 * 32 * 4;
@@ -214,15 +212,15 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
   constexpr bool Q_IN_REGS = NT * HDP <= 128;
   extern __shared__ __align__(128) char smem[];
   const int cols = a.rows_per * a.heads_per;            // live columns at most
-  const Q8Smem at = q8_smem(Shape::STAGE, LDS, LDQ, a.stages, cols, a.n_items);
-  float* sm_acc = reinterpret_cast<float*>(smem + at.join);          // [warp][min(cols, 8)][LDS]
+  const Q8Smem at = q8_smem(Shape::STAGE, LDS, LDQ, a.stages, cols, a.join_cols, a.n_items);
+  float* sm_acc = reinterpret_cast<float*>(smem + at.join);          // [warp][join_cols][LDS]
   float* sm_m = reinterpret_cast<float*>(smem + at.stats);           // [warp][8]
   float* sm_l = sm_m + Q8_WARPS * 8;                                 // [warp][8]
   int8_t* sm_q = reinterpret_cast<int8_t*>(smem + at.queries);       // [3][cols][LDQ] the queries' bytes, the highest first
   float* sm_f = reinterpret_cast<float*>(smem + at.columns);         // [32] a query's power of two, [32] maximum and [32] sum of merged pieces
   float* sm_w = sm_f + 32;
   int* sm_i = reinterpret_cast<int*>(smem + at.ints);                // [8]
-  int* before = reinterpret_cast<int*>(smem + at.items);             // [n_items + 1] units of the items before this one
+  int* before = reinterpret_cast<int*>(smem + at.items);             // [n_items + 1] tiles of the items before this one
   int* item_row = before + a.n_items + 1;                            // [n_items] first row; request or rows; first position
   int* item_seq = item_row + a.n_items;
   int* item_pos = item_seq + a.n_items;
@@ -233,14 +231,14 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
 
-  // the items' units, summed up
+  // the items' tiles, summed up
   int total = 0;
   for (int i0 = 0; i0 < a.n_items; i0 += Q8_THREADS) {
     const int i = i0 + tid;
     int n = 0;
     if (i < a.n_items) {
       const Q8Item it = q8_item(a, i);
-      if (it.n_rows > 0) n = Q8_PAIR + (q8_span<EXT>(a, it).tiles + UNIT - 1) / UNIT;      // a row without keys has its zeros written too
+      if (it.n_rows > 0) n = Q8_PAIR + q8_span<EXT>(a, it).tiles;      // a row without keys has its zeros written too
       item_row[i] = it.row0;
       item_seq[i] = a.cu_rows ? it.n_rows : it.seq;
       item_pos[i] = it.pos0;
@@ -266,9 +264,11 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
   __syncthreads();
   const int n_hg = a.n_kv_head * a.head_blocks, group = a.n_head / a.n_kv_head;
   if (total == 0) return;
-  const long long all = (long long)total * n_hg, per = max((all + gridDim.x - 1) / gridDim.x, (long long)Q8_MERGE);
-  const int slack = (int)min(per - 1, (long long)Q8_MERGE);
-  // the item in which unit `rem` of a head lies: the last one that begins at or before it
+  // at least two rounds of the warps to a block; cuts are moved by up to three rounds (a merge takes about as long), by less where a block
+  // has much to do, for all wait for the one that got more
+  const long long all = (long long)total * n_hg, per = max((all + gridDim.x - 1) / gridDim.x, 2LL * UNIT);
+  const int slack = (int)min(per <= 6 * UNIT ? per - 1 : max(per / 16, (long long)Q8_PAIR), 3LL * UNIT);
+  // the item in which tile `rem` of a head lies: the last one that begins at or before it
   auto item_at = [&](int rem) {
     int lo = 0, hi = a.n_items - 1;
     while (lo < hi) {
@@ -286,29 +286,29 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
   const long long w_end = cut((blockIdx.x + 1) * per);
   if (w_at >= w_end) return;
 
-  // A block's part of one item's keys under the heads that share a key/value head: units u0 .. u1 - 1.
+  // A block's part of one item's keys under the heads that share a key/value head: from tile `from` to end_tile.
   struct Piece {
     Q8Item it;
     Q8Span span;
-    int hg, hk, h0, n_h, item, u0, u1, end_tile;
+    int hg, hk, h0, n_h, item, from, end_tile;
     bool begins, ends;      // whether the item does with it
     const int* bt;
     const int8_t *k_lane, *v_lane;      // FAST: the lane's piece of the head's first row, and its scale
     const float* s_lane;
   };
-  int at_hg = (int)(w_at / total), at_item = item_at((int)(w_at % total)), at_unit = (int)(w_at % total) - before[at_item];
+  int at_hg = (int)(w_at / total), at_item = item_at((int)(w_at % total)), at_tile = (int)(w_at % total) - before[at_item];
   auto find_piece = [&](Piece& p) {
-    const int lo = at_item, slots = before[lo + 1] - before[lo], to = (int)min((long long)slots, at_unit + (w_end - w_at));
+    const int lo = at_item, slots = before[lo + 1] - before[lo], to = (int)min((long long)slots, at_tile + (w_end - w_at));
     p.hg = at_hg;
     p.item = lo;
-    p.begins = at_unit == 0;
+    p.begins = at_tile == 0;
     p.ends = to == slots;
-    p.u0 = p.begins ? 0 : at_unit - Q8_PAIR;
-    p.u1 = max(to - Q8_PAIR, 0);
-    w_at += to - at_unit;
-    at_unit = to;
+    p.from = p.begins ? 0 : at_tile - Q8_PAIR;
+    p.end_tile = to - Q8_PAIR;
+    w_at += to - at_tile;
+    at_tile = to;
     if (p.ends) {
-      at_unit = 0;
+      at_tile = 0;
       do {
         if (++at_item == a.n_items) {
           at_item = 0;
@@ -326,7 +326,6 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
     p.h0 = p.hk * group + hb * a.heads_per;
     p.n_h = min(a.heads_per, group - hb * a.heads_per);
     p.bt = a.block_table + (size_t)max(p.it.seq, 0) * a.max_blocks;
-    p.end_tile = min(p.u1 * UNIT, p.span.tiles);
     if constexpr (FAST) {
       const long long first = (long long)p.hk * a.ps;
       p.k_lane = a.kc + first * HDP + lane * 16;
@@ -422,7 +421,7 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
     fill = fill + Shape::STAGE == ring_end ? ring : fill + Shape::STAGE;
   };
   auto ask_first = [&](const Piece& p) {      // all stages but one
-    const int tile = p.u0 * UNIT + warp * TPW;
+    const int tile = p.from + warp * TPW;
     if (FAST && tile < p.end_tile) find_pages(p, tile);
     for (int s = 0; s < a.stages - 1; ++s) {
       ask(p, tile + s * UNIT);
@@ -509,7 +508,7 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
       l_run[nt][0] = l_run[nt][1] = ref[nt][0] = ref[nt][1] = 0.f;
     }
 
-    for (int tile = cur.u0 * UNIT + warp * TPW; tile < cur.end_tile; tile += UNIT) {
+    for (int tile = cur.from + warp * TPW; tile < cur.end_tile; tile += UNIT) {
       // the oldest stage has arrived, and every lane is done with the one before it, which is filled again
       if (a.stages == 2) copies_wait<0>();
       else copies_wait<1>();
@@ -705,34 +704,37 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
       ask_first(cur);
     }
 
-    // the warps' results joined, eight columns at a time
+    // the warps' results joined, a few columns at a time
     const bool alone = done.begins && done.ends;
-    float* mine = a.part + (size_t)(2 * blockIdx.x + done.begins) * NQ * (HDP + 2);
+    float* mine = a.part + (size_t)(2 * blockIdx.x + done.begins) * NQ * (HDP + 4);      // a column: HDP sums, the maximum, the denominator
     // entry i of a query's row in shared memory is [pair of dims j][lane g][2]: the dim
     auto dim_of = [&](int i) { return ((i >> 1) & 7) * (HDP / 8) + (i >> 4) * 2 + (i & 1); };
-    const int jq = min(cols, 8);
+    const int jq = a.join_cols;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      if (nt * 8 < live) {
-        if (nt > 0) __syncthreads();
+      for (int q0 = 0; q0 < 8 && nt * 8 + q0 < live; q0 += jq) {
+        if (nt + q0 > 0) __syncthreads();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float l = l_run[nt][c];
+          const int q = 2 * t + c;
+          if (q0 == 0) {
+            float l = l_run[nt][c];
 #pragma unroll
-          for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-          if (g == 0) {
-            sm_m[warp * 8 + 2 * t + c] = m_run[nt][c];
-            sm_l[warp * 8 + 2 * t + c] = l;
+            for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+            if (g == 0) {
+              sm_m[warp * 8 + q] = m_run[nt][c];
+              sm_l[warp * 8 + q] = l;
+            }
           }
-          if (nt * 8 + 2 * t + c < live) {
-            float* dst = sm_acc + (size_t)(warp * jq + 2 * t + c) * LDS + g * 2;
+          if (nt * 8 + q < live && q >= q0 && q < q0 + jq) {
+            float* dst = sm_acc + (size_t)(warp * jq + q - q0) * LDS + g * 2;
 #pragma unroll
             for (int j = 0; j < KS; ++j) *reinterpret_cast<float2*>(dst + j * 16) = make_float2(o[nt][j][c], o[nt][j][2 + c]);
           }
         }
         __syncthreads();
-        for (int x = tid; x < min(live - nt * 8, 8) * HDP; x += Q8_THREADS) {
-          const int mq = x / HDP, i = x % HDP, m = nt * 8 + mq, d = dim_of(i);
+        for (int x = tid; x < min(live - nt * 8 - q0, jq) * HDP; x += Q8_THREADS) {
+          const int mq = q0 + x / HDP, i = x % HDP, m = nt * 8 + mq, d = dim_of(i);
           float mw[Q8_WARPS], M = -INFINITY, l = 0.f, v = 0.f;
 #pragma unroll
           for (int w = 0; w < Q8_WARPS; ++w) {
@@ -742,7 +744,7 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
 #pragma unroll
           for (int w = 0; w < Q8_WARPS; ++w) {
             const float f = mw[w] == -INFINITY && M != -INFINITY ? 0.f : ex2(mw[w] - (M == -INFINITY ? 0.f : M));
-            v = fmaf(f, sm_acc[(size_t)(w * jq + mq) * LDS + i], v);
+            v = fmaf(f, sm_acc[(size_t)(w * jq + mq - q0) * LDS + i], v);
             l = fmaf(f, sm_l[w * 8 + mq], l);
           }
           if (alone) {
@@ -755,11 +757,11 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
             }
             if (d < hd) from_f32(static_cast<TT*>(a.out)[(size_t)(done.it.row0 + row_in(m)) * a.out_ld + h * hd + d], l == 0.f ? 0.f : v * keep1 / l);
           } else {
-            float* p = mine + m * (HDP + 2);
-            p[2 + i] = v;
+            float* p = mine + m * (HDP + 4);
+            p[i] = v;
             if (i == 0) {
-              p[0] = M;
-              p[1] = l;
+              p[HDP] = M;
+              p[HDP + 1] = l;
             }
           }
         }
@@ -769,47 +771,85 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
       // the cuts that were left inside the item; the piece behind cut c is block c's, the first piece that of the block before
       const long long begin = (long long)done.hg * total + before[done.item], end = begin + before[done.item + 1] - before[done.item];
       const int b_first = (int)((begin + slack) / per), n_pieces = (int)((end - slack - 1) / per) - b_first + 1;
-      __threadfence();
       __syncthreads();
-      unsigned* counter = a.counters + (size_t)done.item * n_hg + done.hg;
-      if (tid == 0) sm_i[0] = atomicAdd(counter, 1u) == (unsigned)(n_pieces - 1);
+      if (tid == 0) {      // (the barrier puts the block's stores before this thread's fence)
+        unsigned* counter = a.counters + (size_t)done.item * n_hg + done.hg;
+        __threadfence();
+        const bool last = atomicAdd(counter, 1u) == (unsigned)(n_pieces - 1);
+        sm_i[0] = last;
+        if (last) *counter = 0;
+        __threadfence();
+      }
       __syncthreads();
       if (sm_i[0]) {
-        __threadfence();
-        auto piece = [&](int b) { return a.part + (size_t)(2 * (b_first + b) + (b == 0)) * NQ * (HDP + 2); };
-        // every query's maximum and sum over the pieces first
+        auto piece = [&](int b) { return a.part + (size_t)(2 * (b_first + b) + (b == 0)) * NQ * (HDP + 4); };
+        // every column's maximum and denominator over the pieces first
         for (int m = warp; m < live; m += Q8_WARPS) {
           float M = -INFINITY, l = 0.f;
-          for (int b = lane; b < n_pieces; b += 32) M = fmaxf(M, load_float(piece(b) + m * (HDP + 2)));
-          M = warp_max(M);
-          const float sk = a.sinks ? a.sinks[done.h0 + m - row_in(m) * n_h] * LOG2E : -INFINITY, mm = fmaxf(M, sk), r = mm == -INFINITY ? 0.f : mm;
-          for (int b = lane; b < n_pieces; b += 32) l = fmaf(ex2(load_float(piece(b) + m * (HDP + 2)) - r), load_float(piece(b) + m * (HDP + 2) + 1), l);
-          l = warp_sum(l) + (a.sinks ? ex2(sk - r) : 0.f);
+          for (int b = lane; b < n_pieces; b += 32) {
+            const float* p = piece(b) + m * (HDP + 4) + HDP;
+            const float pm = load_float(p), pl = load_float(p + 1), top = fmaxf(M, pm), r = top == -INFINITY ? 0.f : top;
+            l = fmaf(l, ex2(M - r), pl * ex2(pm - r));
+            M = top;
+          }
+          const float sk = a.sinks ? a.sinks[done.h0 + m - row_in(m) * n_h] * LOG2E : -INFINITY, mm = fmaxf(warp_max(M), sk), r = mm == -INFINITY ? 0.f : mm;
+          l = warp_sum(l * ex2(M - r)) + (a.sinks ? ex2(sk - r) : 0.f);
           if (lane == 0) {
             sm_w[m] = r;
             sm_w[32 + m] = l;
           }
         }
         __syncthreads();
-        for (int x = tid; x < live * HDP; x += Q8_THREADS) {
-          const int m = x / HDP, i = x % HDP, d = dim_of(i);
-          const float r = sm_w[m], l = sm_w[32 + m];
-          float v = 0.f;
-          for (int b0 = 0; b0 < n_pieces; b0 += 8) {      // eight in flight
-            float pm[8], pv[8];
+        // four entries of a column to a thread, eight pieces in flight; with few columns the pieces go to several groups of threads
+        const int quads = live * (HDP / 4), groups = min(max(Q8_THREADS / quads, 1), n_pieces > 8 ? Q8_WARPS : 1);
+        for (int x0 = 0; x0 < quads * groups; x0 += Q8_THREADS) {
+          const int x = x0 + tid, part = x / quads, q = x - part * quads, m = q / (HDP / 4), i = q % (HDP / 4) * 4;
+          float v[4] = {0.f, 0.f, 0.f, 0.f};
+          if (part < groups) {
+            const float r = sm_w[m];
+            const int from = n_pieces * part / groups, to = n_pieces * (part + 1) / groups;
+            for (int b0 = from; b0 < to; b0 += 8) {
+              float pm[8];
+              float4 pv[8];
 #pragma unroll
-            for (int b = 0; b < 8; ++b) {
-              const float* p = piece(min(b0 + b, n_pieces - 1)) + m * (HDP + 2);
-              pm[b] = load_float(p);
-              pv[b] = load_float(p + 2 + i);
+              for (int b = 0; b < 8; ++b) {
+                const float* p = piece(min(b0 + b, to - 1)) + m * (HDP + 4);
+                pm[b] = load_float(p + HDP);
+                asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(pv[b].x), "=f"(pv[b].y), "=f"(pv[b].z), "=f"(pv[b].w) : "l"(p + i) : "memory");
+              }
+#pragma unroll
+              for (int b = 0; b < 8; ++b)
+                if (b0 + b < to) {
+                  const float w = ex2(pm[b] - r);
+                  v[0] = fmaf(w, pv[b].x, v[0]);
+                  v[1] = fmaf(w, pv[b].y, v[1]);
+                  v[2] = fmaf(w, pv[b].z, v[2]);
+                  v[3] = fmaf(w, pv[b].w, v[3]);
+                }
             }
-#pragma unroll
-            for (int b = 0; b < 8; ++b) v = b0 + b < n_pieces ? fmaf(ex2(pm[b] - r), pv[b], v) : v;
           }
-          const int h = done.h0 + m - row_in(m) * n_h;
-          if (d < hd) from_f32(static_cast<TT*>(a.out)[(size_t)(done.it.row0 + row_in(m)) * a.out_ld + h * hd + d], l == 0.f ? 0.f : v / l);
+          if (groups > 1) {       // one round of threads then: the groups' sums are added in their order
+            float4* sum = reinterpret_cast<float4*>(sm_acc);
+            if (part > 0 && part < groups) sum[x - quads] = make_float4(v[0], v[1], v[2], v[3]);
+            __syncthreads();
+            if (part > 0) continue;
+            for (int k = 0; k < groups - 1; ++k) {
+              const float4 o4 = sum[k * quads + q];
+              v[0] += o4.x;
+              v[1] += o4.y;
+              v[2] += o4.z;
+              v[3] += o4.w;
+            }
+          }
+          if (part < groups) {
+            const float l = sm_w[32 + m];
+            const int h = done.h0 + m - row_in(m) * n_h;
+            TT* out = static_cast<TT*>(a.out) + (size_t)(done.it.row0 + row_in(m)) * a.out_ld + h * hd;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (dim_of(i + e) < hd) from_f32(out[dim_of(i + e)], l == 0.f ? 0.f : v[e] / l);
+          }
         }
-        if (tid == 0) *counter = 0;
       }
     }
     if (!more) break;
@@ -819,7 +859,7 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
 
 // How a launch is laid out.
 struct Q8Plan {
-  int hdp, nt, heads_per, head_blocks, rows_per, tiles_per_seg, stages, smem;
+  int hdp, nt, heads_per, head_blocks, rows_per, tiles_per_seg, stages, join_cols, smem;
   long long items, blocks, floats, counters;
 };
 
