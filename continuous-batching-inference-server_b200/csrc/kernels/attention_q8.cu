@@ -1,5 +1,6 @@
 // Launcher of the attention over the 8-bit cache (attention_q8.cuh).
 #include "attention_q8.cuh"
+#include <string.h>
 
 namespace cbis {
 extern template int q8_run<32>(const Q8Args&, const Q8Plan&, bool, int, cudaStream_t);
@@ -77,13 +78,20 @@ CBIS_EXPORT int cbis_attention_q8_scratch(int n, int rows_of_seg, int n_head, in
 // rows_of_seg 0: n decoding rows (row_seq, positions; with k_off >= 0 the current token's key and value are taken from q's rows, quantised
 // and stored at slot_mapping[row]); else the n requests from seg0 on, whose rows are cu_rows[s] .. cu_rows[s + 1] - 1 at positions from
 // seg_start[s] on.  A row whose request is no row of the block table, or that sees no key, gets zeros.
-CBIS_EXPORT int cbis_attention_q8(const void* q, int ld, int k_off, int v_off, void* kc, void* ks, void* vc, void* vs, const int* block_table,
-                                  int max_blocks, int n_seqs, int num_pages, const int* row_seq, const int* positions,
-                                  const int* slot_mapping, const int* cu_rows, const int* seg_start, int seg0, int n, int rows_of_seg, int n_rows,
-                                  void* out, int out_ld, float* part, long long part_floats, unsigned* counters, long long n_counters,
-                                  int n_head, int n_kv_head, int hd, int ps, float scale, int window, int max_context, int dtype,
-                                  void* stream, const float* sinks, const float* slopes, const float* rates, float temp_coef,
-                                  int temp_every, float cap, int keep) {
+// The call is one record of 8-byte fields.
+struct Q8Call {
+  long long q, ld, k_off, v_off, kc, ks, vc, vs, block_table, max_blocks, n_seqs, num_pages, row_seq, positions, slot_mapping, cu_rows, seg_start,
+      seg0, n, rows_of_seg, n_rows, out, out_ld, part, part_floats, counters, n_counters, n_head, n_kv_head, hd, ps, window, max_context, dtype,
+      stream, sinks, slopes, rates, temp_every, keep;
+  double scale, temp_coef, cap;
+};
+CBIS_EXPORT int cbis_attention_q8(const void* call) {
+  Q8Call x;
+  memcpy(&x, call, sizeof x);
+  const int n = (int)x.n, rows_of_seg = (int)x.rows_of_seg, dtype = (int)x.dtype, hd = (int)x.hd, ps = (int)x.ps, n_head = (int)x.n_head,
+            n_kv_head = (int)x.n_kv_head, max_blocks = (int)x.max_blocks, num_pages = (int)x.num_pages, n_seqs = (int)x.n_seqs,
+            max_context = (int)x.max_context, keep = (int)x.keep, window = (int)x.window, n_rows = (int)x.n_rows, seg0 = (int)x.seg0, ld = (int)x.ld;
+  float* part = (float*)x.part;
   if (n <= 0) return CBIS_OK;
   if (dtype != CBIS_F32 && dtype != CBIS_BF16) return CBIS_ERR_BAD_DTYPE;
   if (hd <= 0 || hd > 256 || hd % 16 || ps <= 0 || n_kv_head <= 0 || n_head <= 0 || n_head % n_kv_head || max_blocks <= 0 || keep < 0 ||
@@ -92,25 +100,27 @@ CBIS_EXPORT int cbis_attention_q8(const void* q, int ld, int k_off, int v_off, v
   if ((long long)max_blocks * ps >= Q8_MAX_POSITION || (long long)num_pages * ps * n_kv_head > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
   if (window < -Q8_MAX_POSITION) return CBIS_ERR_BAD_SIZE;
   const int f32 = dtype == CBIS_F32, align = f32 ? 4 : 8;
-  if (ld % align || (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15)) return CBIS_ERR_ALIGNMENT;
+  if (ld % align || ((x.q | x.kc | x.vc) & 15)) return CBIS_ERR_ALIGNMENT;
   const Q8Plan p = q8_plan(n, rows_of_seg, n_head, n_kv_head, hd, f32, max_context);
   if (p.items > Q8_MAX_ITEMS || p.items * ((long long)max_blocks * ps / 16 + 8) > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;      // the tiles are counted in 32 bits
   if ((uintptr_t)part & 15) return CBIS_ERR_ALIGNMENT;
-  if (part_floats < p.floats || n_counters < p.counters || (k_off >= 0 && slot_mapping == nullptr)) return CBIS_ERR_BAD_SIZE;
+  if (x.part_floats < p.floats || x.n_counters < p.counters || (x.k_off >= 0 && !x.slot_mapping)) return CBIS_ERR_BAD_SIZE;
   Q8Args a = {};
-  a.q = q; a.out = out; a.kc = (int8_t*)kc; a.vc = (int8_t*)vc; a.ks = (float*)ks; a.vs = (float*)vs;
-  a.block_table = block_table; a.row_seq = row_seq; a.positions = positions; a.slot_mapping = slot_mapping;
-  a.cu_rows = rows_of_seg ? cu_rows : nullptr; a.seg_start = seg_start; a.part = part; a.counters = counters;
-  a.sinks = sinks; a.slopes = slopes; a.rates = rates;
-  a.n_rows = n_rows; a.ld = ld; a.out_ld = out_ld; a.k_off = k_off; a.v_off = v_off; a.max_blocks = max_blocks; a.num_pages = num_pages; a.n_seqs = n_seqs;
+  a.q = (const void*)x.q; a.out = (void*)x.out; a.kc = (int8_t*)x.kc; a.vc = (int8_t*)x.vc; a.ks = (float*)x.ks; a.vs = (float*)x.vs;
+  a.block_table = (const int*)x.block_table; a.row_seq = (const int*)x.row_seq; a.positions = (const int*)x.positions;
+  a.slot_mapping = (const int*)x.slot_mapping;
+  a.cu_rows = rows_of_seg ? (const int*)x.cu_rows : nullptr; a.seg_start = (const int*)x.seg_start; a.part = part; a.counters = (unsigned*)x.counters;
+  a.sinks = (const float*)x.sinks; a.slopes = (const float*)x.slopes; a.rates = (const float*)x.rates;
+  a.n_rows = n_rows; a.ld = ld; a.out_ld = (int)x.out_ld; a.k_off = (int)x.k_off; a.v_off = (int)x.v_off; a.max_blocks = max_blocks; a.num_pages = num_pages; a.n_seqs = n_seqs;
   a.seg0 = seg0; a.n_items = (int)p.items; a.tiles_per_seg = p.tiles_per_seg; a.n_head = n_head; a.n_kv_head = n_kv_head;
   a.heads_per = p.heads_per; a.head_blocks = p.head_blocks; a.rows_per = p.rows_per;
   a.stages = p.stages; a.join_cols = p.join_cols; a.page_rows = n_kv_head * ps; a.hd = hd; a.ps = ps; a.ps_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (ps == 1 << i) a.ps_shift = i;
-  a.window = window; a.keep = keep; a.temp_every = temp_every; a.scale = scale; a.cap = cap; a.temp_coef = temp_coef;
-  const bool ext = cap > 0.f || (keep > 0 && window != 0) || slopes || temp_every > 0;
-  cudaStream_t st = (cudaStream_t)stream;
+  a.window = window; a.keep = keep; a.temp_every = (int)x.temp_every; a.scale = (float)x.scale; a.cap = (float)x.cap;
+  a.temp_coef = (float)x.temp_coef;
+  const bool ext = a.cap > 0.f || (keep > 0 && window != 0) || a.slopes || a.temp_every > 0;
+  cudaStream_t st = (cudaStream_t)x.stream;
   switch (p.hdp) {
     case 32: return q8_run<32>(a, p, ext, f32, st);
     case 64: return q8_run<64>(a, p, ext, f32, st);

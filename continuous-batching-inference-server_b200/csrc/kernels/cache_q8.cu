@@ -3,6 +3,7 @@
 //
 // Both are bound by their bytes once there are some megabytes of them, and by the launch below that.
 #include "cache_q8.cuh"
+#include <string.h>
 
 namespace cbis {
 
@@ -174,9 +175,21 @@ using namespace cbis;
 
 // hd_v 0: the keys' width.  vc null: one array stands for keys and values and takes the rows at k_off.  n_slots: num_pages * ps; rows
 // whose slot is none of these are not written.
-CBIS_EXPORT int cbis_kv_write_q8(const void* qkv, int ld, int k_off, int v_off, void* kc, void* ks, void* vc, void* vs,
-                                 const int* slot_mapping, int n_slots, int T, int heads, int hd, int hd_v, int ps, int dtype,
-                                 void* stream) {
+// The call is one record of 8-byte fields, as below.
+struct KvWriteCall {
+  long long qkv, ld, k_off, v_off, kc, ks, vc, vs, slot_mapping, n_slots, T, heads, hd, hd_v, ps, dtype, stream;
+};
+CBIS_EXPORT int cbis_kv_write_q8(const void* call) {
+  KvWriteCall x;
+  memcpy(&x, call, sizeof x);
+  const void* qkv = (const void*)x.qkv;
+  void *kc = (void*)x.kc, *ks = (void*)x.ks, *vc = (void*)x.vc, *vs = (void*)x.vs, *stream = (void*)x.stream;
+  const int* slot_mapping = (const int*)x.slot_mapping;
+  int hd_v = (int)x.hd_v;
+  const int ld = (int)x.ld, k_off = (int)x.k_off, v_off = (int)x.v_off, T = (int)x.T, heads = (int)x.heads, hd = (int)x.hd, ps = (int)x.ps,
+            dtype = (int)x.dtype;
+  if (x.n_slots > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
+  const int n_slots = (int)x.n_slots;
   if (T <= 0) return CBIS_OK;
   if (hd_v <= 0) hd_v = hd;
   if (heads <= 0 || hd <= 0 || ps <= 0 || n_slots < 0) return CBIS_ERR_BAD_SIZE;
@@ -215,9 +228,19 @@ CBIS_EXPORT int cbis_kv_write_q8(const void* qkv, int ld, int k_off, int v_off, 
 // the tokens that its queries at seg_start[s] .. seg_ctx[s] - 1 see: those from first_seen(seg_start[s]) on, at most max_tokens of
 // them, and the kept first ones.  whole: the rest of these tokens' pages too, up to seg_ctx[s] (a kernel that brings pages in whole
 // multiplies what it masks by zero, which only numbers survive).
-CBIS_EXPORT int cbis_kv_read_q8(const void* kc, const void* ks, const void* vc, const void* vs, void* ko, void* vo, const int* block_table,
-                                int max_blocks, int num_pages, const int* seg_start, const int* seg_ctx, int n_seg, int max_tokens,
-                                int heads, int hd, int hd_v, int ps, int window, int keep, int whole, int dtype, void* stream) {
+struct KvReadCall {
+  long long kc, ks, vc, vs, ko, vo, block_table, max_blocks, num_pages, seg_start, seg_ctx, n_seg, max_tokens, heads, hd, hd_v, ps, window, keep,
+      whole_dtype, stream;      // whole | dtype << 1
+};
+CBIS_EXPORT int cbis_kv_read_q8(const void* call) {
+  KvReadCall x;
+  memcpy(&x, call, sizeof x);
+  const void *kc = (const void*)x.kc, *ks = (const void*)x.ks, *vc = (const void*)x.vc, *vs = (const void*)x.vs;
+  void *ko = (void*)x.ko, *vo = (void*)x.vo, *stream = (void*)x.stream;
+  const int *block_table = (const int*)x.block_table, *seg_start = (const int*)x.seg_start, *seg_ctx = (const int*)x.seg_ctx;
+  int hd_v = (int)x.hd_v;
+  const int max_blocks = (int)x.max_blocks, num_pages = (int)x.num_pages, n_seg = (int)x.n_seg, max_tokens = (int)x.max_tokens, heads = (int)x.heads,
+            hd = (int)x.hd, ps = (int)x.ps, window = (int)x.window, keep = (int)x.keep, whole = (int)x.whole_dtype & 1, dtype = (int)(x.whole_dtype >> 1);
   if (n_seg <= 0 || max_tokens <= 0) return CBIS_OK;
   if (hd_v <= 0) hd_v = hd;
   if (heads <= 0 || hd <= 0 || ps <= 0 || max_blocks <= 0 || keep < 0 || n_seg > 65535) return CBIS_ERR_BAD_SIZE;

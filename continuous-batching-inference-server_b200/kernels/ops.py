@@ -8,6 +8,7 @@ path go to the library GEMM (cuBLASLt through ``torch``), as the reference's go 
 from __future__ import annotations
 
 import ctypes
+import struct
 import weakref
 from ctypes import c_float, c_int, c_void_p
 from typing import NamedTuple, Optional
@@ -556,23 +557,35 @@ def q8_pages(num_pages: int, heads: int, page_size: int, width: int, device="cud
                    torch.zeros((num_pages, heads, page_size), dtype=torch.float32, device=device))
 
 
+# The calls of the 8-bit cache hand the library one packed record of 8-byte fields: a step of a small model is bound by the host's
+# calls, and forty arguments converted one by one took 10 us of them.  Arguments are looked at in one expression; only if that does not
+# hold are they taken one by one, to say what is wrong.
+_WRITE_Q8, _READ_Q8, _ATTEND_Q8 = struct.Struct("17q"), struct.Struct("21q"), struct.Struct("40q3d")
+_INT8, _INT32, _FLOAT32, _BFLOAT16 = torch.int8, torch.int32, torch.float32, torch.bfloat16
 _q8_fns = {}
 
 
-def _q8_fn(name: str, argtypes):
+def _q8_fn(name: str):
     fn = _q8_fns.get(name)
     if fn is None:
         fn = getattr(kernels(), name)
-        fn.argtypes = argtypes
+        fn.argtypes = [ctypes.c_char_p]
         _q8_fns[name] = fn
     return fn
 
 
-_P, _I, _F, _L = c_void_p, c_int, c_float, ctypes.c_longlong
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def _at(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _stream_int() -> int:
+    if _raw_stream is not None and _raw_device is not None:
+        return _raw_stream(_raw_device())
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _device_now() -> int:
+    return _raw_device() if _raw_device is not None else torch.cuda.current_device()
 
 
 def _q8_need(ok, what: str, why: str) -> None:
@@ -590,9 +603,8 @@ def _q8_here(what: str, *ts) -> None:
             raise KernelError(f"{what}: kernels take CUDA tensors only; there is no CPU path")
         if dev is None:
             dev = t.device
-            here = _raw_device() if _raw_device is not None else torch.cuda.current_device()
-            if dev.index != here:
-                raise KernelError(f"{what}: the tensors are on {dev}, the current device is cuda:{here}")
+            if dev.index != _device_now():
+                raise KernelError(f"{what}: the tensors are on {dev}, the current device is cuda:{_device_now()}")
         elif t.device != dev:
             raise KernelError(f"{what}: tensors on {dev} and {t.device}")
 
@@ -622,25 +634,31 @@ def kv_write_q8(qkv, k_off, v_off, k_pages, v_pages, slot_mapping, n_kv_head, he
     both and takes the rows at k_off."""
     what = "kv_write_q8"
     vd = int(v_head_dim) or head_dim
-    if v_pages is not None and v_pages.codes is k_pages.codes:
-        v_pages = None
+    kc, ks = k_pages
+    vc, vs = (None, None) if v_pages is None or v_pages[0] is kc else v_pages
     T = qkv.shape[0]
     code = dtype_code(qkv.dtype)
-    _q8_need(qkv.dim() == 2 and (T == 0 or qkv.stride(1) == 1) and k_off >= 0 and k_off + n_kv_head * head_dim <= qkv.shape[1]
-             and (v_pages is None or (v_off >= 0 and v_off + n_kv_head * vd <= qkv.shape[1])), what,
-             f"{n_kv_head} heads of {head_dim} and {vd} at columns {k_off} and {v_off} do not lie in rows of {tuple(qkv.shape)}")
-    _q8_array(what, "keys", k_pages, n_kv_head, page_size, head_dim)
-    if v_pages is not None:
-        _q8_array(what, "values", v_pages, n_kv_head, page_size, vd)
-        _q8_need(v_pages.codes.shape[0] == k_pages.codes.shape[0], what, "keys and values have different numbers of pages")
-    _q8_int32(what, "slot_mapping", slot_mapping, T)
-    vc, vs = (None, None) if v_pages is None else v_pages
-    _q8_here(what, qkv, k_pages.codes, k_pages.scales, vc, vs, slot_mapping)
-    if T == 0:
-        return
-    fn = _q8_fn("cbis_kv_write_q8", [_P, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P])
-    st = fn(_at(qkv), qkv.stride(0), k_off, v_off, _at(k_pages.codes), _at(k_pages.scales), _at(vc), _at(vs), _at(slot_mapping),
-            k_pages.codes.shape[0] * page_size, T, n_kv_head, head_dim, vd, page_size, code, _stream())
+    shape, dev, columns = kc.shape, qkv.get_device(), qkv.shape[-1]
+    if not (vc is not None and T > 0 and qkv.dim() == 2 and kc.dtype is _INT8 and vc.dtype is _INT8 and ks.dtype is _FLOAT32 and vs.dtype is _FLOAT32
+            and shape[1:] == (n_kv_head, page_size, head_dim) and vc.shape == (shape[0], n_kv_head, page_size, vd)
+            and ks.shape == shape[:3] and vs.shape == shape[:3] and kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous()
+            and vs.is_contiguous() and slot_mapping.dtype is _INT32 and slot_mapping.is_contiguous() and slot_mapping.numel() >= T
+            and qkv.stride(1) == 1 and 0 <= k_off <= columns - n_kv_head * head_dim and 0 <= v_off <= columns - n_kv_head * vd
+            and 0 <= dev == kc.get_device() == ks.get_device() == vc.get_device() == vs.get_device() == slot_mapping.get_device() == _device_now()):
+        _q8_need(qkv.dim() == 2 and (T == 0 or qkv.stride(1) == 1) and k_off >= 0 and k_off + n_kv_head * head_dim <= columns
+                 and (vc is None or (v_off >= 0 and v_off + n_kv_head * vd <= columns)), what,
+                 f"{n_kv_head} heads of {head_dim} and {vd} at columns {k_off} and {v_off} do not lie in rows of {tuple(qkv.shape)}")
+        _q8_array(what, "keys", k_pages, n_kv_head, page_size, head_dim)
+        if vc is not None:
+            _q8_array(what, "values", v_pages, n_kv_head, page_size, vd)
+            _q8_need(vc.shape[0] == shape[0], what, "keys and values have different numbers of pages")
+        _q8_int32(what, "slot_mapping", slot_mapping, T)
+        _q8_here(what, qkv, kc, ks, vc, vs, slot_mapping)
+        if T == 0:
+            return
+    st = _q8_fn("cbis_kv_write_q8")(_WRITE_Q8.pack(
+        qkv.data_ptr(), qkv.stride(0), k_off, v_off, kc.data_ptr(), ks.data_ptr(), _at(vc), _at(vs), slot_mapping.data_ptr(),
+        shape[0] * page_size, T, n_kv_head, head_dim, vd, page_size, code, _stream_int()))
     _check(st, what, f"T={T} kv_heads={n_kv_head} head_dim={head_dim} page={page_size}")
 
 
@@ -652,35 +670,47 @@ def kv_read_q8(k_pages, v_pages, k_out, v_out, block_table, seg_start, seg_ctx, 
     ``whole_pages``: what the request holds beside them in their pages is read back too; any kernel that takes pages then reads ``k_out`` and
     ``v_out`` through the same block table.  ``v_pages`` None: one array."""
     what = "kv_read_q8"
-    if v_pages is not None and v_pages.codes is k_pages.codes:
-        v_pages = v_out = None
-    _q8_need(k_pages.codes.dim() == 4, what, "the keys' codes are not [pages, heads, page_size, width]")
-    P, G, ps, hd = k_pages.codes.shape
-    _q8_array(what, "keys", k_pages, G, ps, hd)
-    _q8_table(what, block_table)
-    S = block_table.shape[0]
+    kc, ks = k_pages
+    vc, vs = (None, None) if v_pages is None or v_pages[0] is kc else v_pages
     code = dtype_code(k_out.dtype)
-    outs = [(k_out, k_pages)]
-    vd = hd
-    if v_pages is not None:
-        vd = v_pages.codes.shape[-1]
-        _q8_array(what, "values", v_pages, G, ps, vd)
-        outs.append((v_out, v_pages))
-    for o, p in outs:
-        _q8_need(o is not None and o.dtype == k_out.dtype and o.shape == p.codes.shape and p.codes.shape[0] == P and o.is_contiguous(), what,
-                 "the values' pages must be contiguous, of one type and of the codes' shape")
-    _q8_int32(what, "seg_start", seg_start, S)
-    _q8_int32(what, "seg_ctx", seg_ctx, S)
-    _q8_need(keep >= 0, what, "keep is negative")
-    vc, vs = (None, None) if v_pages is None else v_pages
-    _q8_here(what, k_pages.codes, k_pages.scales, vc, vs, k_out, v_out, block_table, seg_start, seg_ctx)
-    if S == 0 or max_tokens <= 0 or P == 0:
+    shape, dev = kc.shape, kc.get_device()
+    S = block_table.shape[0]
+    if not (vc is not None and v_out is not None and len(shape) == 4 and kc.dtype is _INT8 and vc.dtype is _INT8 and ks.dtype is _FLOAT32
+            and vs.dtype is _FLOAT32 and vc.shape[:3] == shape[:3] and len(vc.shape) == 4 and ks.shape == shape[:3] and vs.shape == shape[:3]
+            and k_out.shape == shape and v_out.shape == vc.shape and v_out.dtype is k_out.dtype and kc.is_contiguous() and vc.is_contiguous()
+            and ks.is_contiguous() and vs.is_contiguous() and k_out.is_contiguous() and v_out.is_contiguous() and block_table.dtype is _INT32
+            and block_table.dim() == 2 and block_table.is_contiguous() and block_table.shape[1] > 0 and seg_start.dtype is _INT32 and seg_ctx.dtype is _INT32
+            and seg_start.is_contiguous() and seg_ctx.is_contiguous() and seg_start.numel() >= S and seg_ctx.numel() >= S and keep >= 0
+            and 0 <= dev == ks.get_device() == vc.get_device() == vs.get_device() == k_out.get_device() == v_out.get_device()
+            == block_table.get_device() == seg_start.get_device() == seg_ctx.get_device() == _device_now()):
+        _q8_need(len(shape) == 4, what, "the keys' codes are not [pages, heads, page_size, width]")
+        _q8_array(what, "keys", k_pages, *shape[1:])
+        _q8_table(what, block_table)
+        outs = [(k_out, kc)]
+        if vc is not None:
+            _q8_array(what, "values", v_pages, shape[1], shape[2], vc.shape[-1])
+            outs.append((v_out, vc))
+        for o, c in outs:
+            _q8_need(o is not None and o.dtype == k_out.dtype and o.shape == c.shape and c.shape[0] == shape[0] and o.is_contiguous(), what,
+                     "the values' pages must be contiguous, of one type and of the codes' shape")
+        _q8_int32(what, "seg_start", seg_start, S)
+        _q8_int32(what, "seg_ctx", seg_ctx, S)
+        _q8_need(keep >= 0, what, "keep is negative")
+        if vc is None:
+            v_out = None
+        _q8_here(what, kc, ks, vc, vs, k_out, v_out, block_table, seg_start, seg_ctx)
+    if S == 0 or max_tokens <= 0 or shape[0] == 0:
         return
-    fn = _q8_fn("cbis_kv_read_q8", [_P, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P])
-    st = fn(_at(k_pages.codes), _at(k_pages.scales), _at(vc), _at(vs), _at(k_out), _at(v_out) if v_pages is not None else None,
-            _at(block_table), block_table.shape[1], P, _at(seg_start), _at(seg_ctx), S, int(max_tokens), G, hd, vd, ps, int(window),
-            int(keep), int(bool(whole_pages)), code, _stream())
-    _check(st, what, f"requests={S} heads={G} widths={hd}/{vd} page={ps}")
+    _kv_read_q8(kc, ks, vc, vs, k_out, v_out, block_table.data_ptr(), block_table.shape[1], seg_start.data_ptr(), seg_ctx.data_ptr(), S,
+                int(max_tokens), int(window), int(keep), bool(whole_pages), code)
+
+
+def _kv_read_q8(kc, ks, vc, vs, k_out, v_out, table: int, blocks: int, start: int, ctx: int, n: int, max_tokens, window, keep, whole, code):
+    P, G, ps, hd = kc.shape
+    st = _q8_fn("cbis_kv_read_q8")(_READ_Q8.pack(
+        kc.data_ptr(), ks.data_ptr(), _at(vc), _at(vs), k_out.data_ptr(), _at(v_out), table, blocks, P, start, ctx, n, max_tokens, G, hd,
+        hd if vc is None else vc.shape[3], ps, window, keep, int(whole) | code << 1, _stream_int()))
+    _check(st, "kv_read_q8", f"requests={n} heads={G} width={hd} page={ps}")
 
 
 ATTENTION_Q8_MAX_HEAD_DIM = 256
@@ -693,9 +723,10 @@ def attention_q8_takes(head_dim: int, v_head_dim: int = 0) -> bool:
 
 
 def _q8_scratch(n, rows_of_seg, n_head, n_kv_head, head_dim, code, max_context):
-    fn = _q8_fn("cbis_attention_q8_scratch", [_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_L), ctypes.POINTER(_L)])
-    floats, counters = _L(), _L()
-    return fn(n, rows_of_seg, n_head, n_kv_head, head_dim, code, max_context, ctypes.byref(floats), ctypes.byref(counters)), floats.value, counters.value
+    fn = kernels().cbis_attention_q8_scratch
+    floats, counters = ctypes.c_longlong(), ctypes.c_longlong()
+    return (fn(c_int(n), c_int(rows_of_seg), c_int(n_head), c_int(n_kv_head), c_int(head_dim), c_int(code), c_int(max_context),
+               ctypes.byref(floats), ctypes.byref(counters)), floats.value, counters.value)
 
 
 def attention_q8_scratch(rows: int, max_seg_rows: int, n_seg: int, n_head: int, n_kv_head: int, head_dim: int, max_context: int, dtype):
@@ -720,6 +751,22 @@ def _prefill_q8_chunks(max_seg_rows, n_seg, n_head, head_dim, max_context, dtype
     return prefill_key_chunks(-(-max_seg_rows // 64), n_head, n_seg, max_context, 1, 8 if dtype == torch.bfloat16 else 16)
 
 
+def _q8_attention_ok(q, kc, ks, vc, vs, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, slopes, sinks, rates, keep) -> bool:
+    shape, dev = kc.shape, q.get_device()
+    return (head_dim % 16 == 0 and 16 <= head_dim <= ATTENTION_Q8_MAX_HEAD_DIM and n_kv_head > 0 and n_head > 0 and n_head % n_kv_head == 0
+            and kc.dtype is _INT8 and vc.dtype is _INT8 and ks.dtype is _FLOAT32 and vs.dtype is _FLOAT32
+            and shape[1:] == (n_kv_head, page_size, head_dim) and vc.shape == shape and ks.shape == shape[:3] and vs.shape == shape[:3]
+            and kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
+            and block_table.dtype is _INT32 and block_table.dim() == 2 and block_table.is_contiguous() and block_table.shape[1] > 0
+            and q.dim() == 2 and q.stride(1) == 1 and q.shape[1] >= n_head * head_dim and out.dim() == 2 and out.dtype is q.dtype
+            and out.stride(1) == 1 and out.shape[0] >= q.shape[0] and out.shape[1] >= n_head * head_dim
+            and scratch.dtype is _FLOAT32 and scratch.is_contiguous() and counters.dtype is _INT32 and counters.is_contiguous()
+            and slopes is None and rates is None and keep >= 0
+            and (sinks is None or (sinks.dtype is _FLOAT32 and sinks.numel() == n_head and sinks.is_contiguous() and sinks.get_device() == dev))
+            and 0 <= dev == kc.get_device() == ks.get_device() == vc.get_device() == vs.get_device() == block_table.get_device() == out.get_device()
+            == scratch.get_device() == counters.get_device() == _device_now())
+
+
 def _q8_attention_checks(what, q, k_pages, v_pages, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, slopes,
                          sinks, rates, keep):
     _q8_need(attention_q8_takes(head_dim), what, f"head_dim={head_dim} is no multiple of 16 up to {ATTENTION_Q8_MAX_HEAD_DIM}")
@@ -742,14 +789,16 @@ def _q8_attention_checks(what, q, k_pages, v_pages, block_table, out, scratch, c
 def _attention_q8(what, q, k_off, v_off, k_pages, v_pages, block_table, row_seq, positions, slot_mapping, cu_rows, seg_start, seg0, n,
                   rows_of_seg, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, scale, window, max_context, slopes, sinks,
                   q_temp, rates, cap, keep):
-    fn = _q8_fn("cbis_attention_q8", [_P, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _P, _L, _P, _L,
-                                      _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _P, _P, _F, _I, _F, _I])
     coef, every = q_temp if q_temp else (0.0, 0)
-    st = fn(_at(q), q.stride(0), k_off, v_off, _at(k_pages.codes), _at(k_pages.scales), _at(v_pages.codes), _at(v_pages.scales),
-            _at(block_table), block_table.shape[1], block_table.shape[0], k_pages.codes.shape[0], _at(row_seq), _at(positions),
-            _at(slot_mapping), _at(cu_rows), _at(seg_start), seg0, n, rows_of_seg, q.shape[0], _at(out), out.stride(0), _at(scratch),
-            scratch.numel(), _at(counters), counters.numel(), n_head, n_kv_head, head_dim, page_size, scale, window, max_context,
-            dtype_code(q.dtype), _stream(), _at(sinks), _at(slopes), _at(rates), coef, int(every), cap, keep)
+    kc, ks = k_pages
+    vc, vs = v_pages
+    seqs, blocks = block_table.shape
+    st = _q8_fn("cbis_attention_q8")(_ATTEND_Q8.pack(
+        q.data_ptr(), q.stride(0), k_off, v_off, kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), block_table.data_ptr(), blocks, seqs,
+        kc.shape[0], _at(row_seq), _at(positions), _at(slot_mapping), _at(cu_rows), _at(seg_start), seg0, n, rows_of_seg, q.shape[0],
+        out.data_ptr(), out.stride(0), scratch.data_ptr(), scratch.numel(), counters.data_ptr(), counters.numel(), n_head, n_kv_head, head_dim,
+        page_size, window, max_context, F32 if q.dtype is _FLOAT32 else BF16, _stream_int(), _at(sinks), _at(slopes), _at(rates), int(every),
+        keep, scale, coef, cap))
     _check(st, what, f"rows={q.shape[0]} heads={n_head}/{n_kv_head} head_dim={head_dim} page={page_size}")
 
 
@@ -764,20 +813,30 @@ def paged_decode_q8(qkv, k_off, v_off, k_pages, v_pages, block_table, row_seq, p
     what = "paged_decode_q8"
     rows = qkv.shape[0]
     dtype_code(qkv.dtype)
-    _q8_attention_checks(what, qkv, k_pages, v_pages, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, slopes,
-                         sinks, rates, keep)
-    _q8_int32(what, "row_seq", row_seq, rows)
-    _q8_int32(what, "positions", positions, rows)
-    if k_off >= 0:
-        wide = n_kv_head * head_dim
-        _q8_need(v_off >= 0 and max(k_off, v_off) + wide <= qkv.shape[1], what, f"keys and values of {wide} do not lie in rows of {tuple(qkv.shape)}")
-        _q8_int32(what, "slot_mapping", slot_mapping, rows)
-    _q8_here(what, qkv, *k_pages, *v_pages, block_table, row_seq, positions, slot_mapping, out, scratch, counters, slopes, sinks, rates)
-    if rows == 0:
-        return
-    _attention_q8(what, qkv, k_off, v_off, k_pages, v_pages, block_table, row_seq, positions, slot_mapping, None, None, 0, rows, 0, out,
-                  scratch, counters, n_head, n_kv_head, head_dim, page_size, scale, int(window), int(max_context), slopes, sinks, q_temp,
-                  rates, float(cap), int(keep))
+    kc, ks = k_pages
+    vc, vs = v_pages
+    if not (rows > 0 and _q8_attention_ok(qkv, kc, ks, vc, vs, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size,
+                                          slopes, sinks, rates, keep)
+            and row_seq.dtype is _INT32 and positions.dtype is _INT32 and row_seq.is_contiguous() and positions.is_contiguous()
+            and row_seq.numel() >= rows and positions.numel() >= rows and qkv.get_device() == row_seq.get_device() == positions.get_device()
+            and (k_off < 0 or (v_off >= 0 and max(k_off, v_off) + n_kv_head * head_dim <= qkv.shape[1] and slot_mapping is not None
+                               and slot_mapping.dtype is _INT32 and slot_mapping.is_contiguous() and slot_mapping.numel() >= rows
+                               and slot_mapping.get_device() == qkv.get_device()))):
+        _q8_attention_checks(what, qkv, k_pages, v_pages, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, slopes,
+                             sinks, rates, keep)
+        _q8_int32(what, "row_seq", row_seq, rows)
+        _q8_int32(what, "positions", positions, rows)
+        if k_off >= 0:
+            wide = n_kv_head * head_dim
+            _q8_need(v_off >= 0 and max(k_off, v_off) + wide <= qkv.shape[1], what, f"keys and values of {wide} do not lie in rows of {tuple(qkv.shape)}")
+            _q8_int32(what, "slot_mapping", slot_mapping, rows)
+        _q8_here(what, qkv, kc, ks, vc, vs, block_table, row_seq, positions, slot_mapping if k_off >= 0 else None, out, scratch, counters,
+                 slopes, sinks, rates)
+        if rows == 0:
+            return
+    _attention_q8(what, qkv, k_off, v_off, k_pages, v_pages, block_table, row_seq, positions, slot_mapping if k_off >= 0 else None, None, None,
+                  0, rows, 0, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, scale, int(window), int(max_context), slopes,
+                  sinks, q_temp, rates, float(cap), int(keep))
 
 
 def prefill_q8_reads_back(max_seg_rows: int, n_head: int, n_kv_head: int, head_dim: int, page_size: int, dtype, slopes=None, sinks=None,
@@ -800,19 +859,31 @@ def paged_prefill_q8(q, k_pages, v_pages, block_table, cu_rows, seg_start, seg_c
     attended to there.  Without ``work`` the first takes all.  The rest as in ``paged_decode_q8``."""
     what = "paged_prefill_q8"
     dtype_code(q.dtype)
-    _q8_attention_checks(what, q, k_pages, v_pages, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, slopes,
-                         sinks, rates, keep)
-    _q8_need(seg0 >= 0 and n_seg >= 0 and seg0 + n_seg <= block_table.shape[0], what, f"requests {seg0}..{seg0 + n_seg} are not in the block table")
-    _q8_need(row0 >= 0 and n_rows >= 0 and row0 + n_rows <= q.shape[0], what, f"rows {row0}..{row0 + n_rows} are not in q")
-    _q8_int32(what, "cu_rows", cu_rows, seg0 + n_seg + 1)
-    _q8_int32(what, "seg_start", seg_start, seg0 + n_seg)
-    _q8_int32(what, "seg_ctx", seg_ctx, seg0 + n_seg)
-    _q8_int32(what, "positions", positions, row0 + n_rows)
-    if work is not None:
-        for o, p in zip(work, (k_pages, v_pages)):
-            _q8_need(o.dtype == q.dtype and o.shape == p.codes.shape and o.is_contiguous(), what, "work must be contiguous, of q's type and the codes' shape")
-    _q8_here(what, q, *k_pages, *v_pages, block_table, cu_rows, seg_start, seg_ctx, positions, out, scratch, counters, slopes, sinks, rates,
-             *(work or ()))
+    kc, ks = k_pages
+    vc, vs = v_pages
+    if not (_q8_attention_ok(q, kc, ks, vc, vs, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, slopes, sinks, rates, keep)
+            and seg0 >= 0 and n_seg >= 0 and seg0 + n_seg <= block_table.shape[0] and row0 >= 0 and n_rows >= 0 and row0 + n_rows <= q.shape[0]
+            and cu_rows.dtype is _INT32 and seg_start.dtype is _INT32 and seg_ctx.dtype is _INT32 and positions.dtype is _INT32
+            and cu_rows.is_contiguous() and seg_start.is_contiguous() and seg_ctx.is_contiguous() and positions.is_contiguous()
+            and cu_rows.numel() > seg0 + n_seg and seg_start.numel() >= seg0 + n_seg and seg_ctx.numel() >= seg0 + n_seg
+            and positions.numel() >= row0 + n_rows
+            and q.get_device() == cu_rows.get_device() == seg_start.get_device() == seg_ctx.get_device() == positions.get_device()
+            and (work is None or (work[0].dtype is q.dtype and work[1].dtype is q.dtype and work[0].shape == kc.shape and work[1].shape == vc.shape
+                                  and work[0].is_contiguous() and work[1].is_contiguous()
+                                  and q.get_device() == work[0].get_device() == work[1].get_device()))):
+        _q8_attention_checks(what, q, k_pages, v_pages, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, slopes,
+                             sinks, rates, keep)
+        _q8_need(seg0 >= 0 and n_seg >= 0 and seg0 + n_seg <= block_table.shape[0], what, f"requests {seg0}..{seg0 + n_seg} are not in the block table")
+        _q8_need(row0 >= 0 and n_rows >= 0 and row0 + n_rows <= q.shape[0], what, f"rows {row0}..{row0 + n_rows} are not in q")
+        _q8_int32(what, "cu_rows", cu_rows, seg0 + n_seg + 1)
+        _q8_int32(what, "seg_start", seg_start, seg0 + n_seg)
+        _q8_int32(what, "seg_ctx", seg_ctx, seg0 + n_seg)
+        _q8_int32(what, "positions", positions, row0 + n_rows)
+        if work is not None:
+            for o, p in zip(work, (k_pages, v_pages)):
+                _q8_need(o.dtype == q.dtype and o.shape == p.codes.shape and o.is_contiguous(), what, "work must be contiguous, of q's type and the codes' shape")
+        _q8_here(what, q, kc, ks, vc, vs, block_table, cu_rows, seg_start, seg_ctx, positions, out, scratch, counters, slopes, sinks, rates,
+                 *(work or ()))
     if n_seg == 0 or n_rows == 0 or max_seg_rows <= 0:
         return
     window, cap, keep = int(window), float(cap), int(keep)
@@ -821,9 +892,10 @@ def paged_prefill_q8(q, k_pages, v_pages, block_table, cu_rows, seg_start, seg_c
                              int(max_seg_rows), out, scratch, counters, n_head, n_kv_head, head_dim, page_size, scale, window,
                              int(max_context), slopes, sinks, q_temp, rates, cap, keep)
     k, v = work
-    segs = slice(seg0, seg0 + n_seg)
     tokens = min(max_context, abs(window) + max_seg_rows) if window else max_context
-    kv_read_q8(k_pages, v_pages, k, v, block_table[segs], seg_start[segs], seg_ctx[segs], tokens, window, keep, whole_pages=True)
+    blocks = block_table.shape[1]
+    _kv_read_q8(kc, ks, vc, vs, k, v, block_table.data_ptr() + 4 * seg0 * blocks, blocks, seg_start.data_ptr() + 4 * seg0,
+                seg_ctx.data_ptr() + 4 * seg0, n_seg, tokens, window, keep, True, F32 if q.dtype is _FLOAT32 else BF16)
     chunks = _prefill_q8_chunks(max_seg_rows, n_seg, n_head, head_dim, max_context, q.dtype)
     args = (q, k, v, block_table, cu_rows, seg_start, out, seg0, n_seg, max_seg_rows, n_head, n_kv_head, head_dim, page_size, scale, window)
     tail = (scratch, positions, row0, n_rows)
@@ -1163,13 +1235,14 @@ def paged_prefill_tc5(q, k_cache, v_cache, block_table, cu_rows, seg_start, out,
     if n_chunks > 1:
         assert partial.dtype == torch.float32 and partial.numel() >= n_rows * n_head * n_chunks * (head_dim + 4)
         assert positions.dtype == torch.int32 and positions.numel() >= row0 + n_rows
-    st = kernels().cbis_paged_prefill_tc5(
-        _ptr(q), c_int(q.stride(0)), c_int(q.shape[0]), _ptr(k_cache), _ptr(v_cache), c_int(k_cache.shape[0]),
-        _ptr(block_table), c_int(block_table.shape[1]), _ptr(cu_rows), _ptr(seg_start), _ptr(out),
-        c_int(out.stride(0)), c_int(seg0), c_int(n_seg), c_int(max_seg_rows), c_int(n_head), c_int(n_kv_head),
-        c_int(head_dim), c_int(page_size), c_float(scale), c_int(window), c_int(n_chunks), c_int(chunk_keys),
-        _ptr(partial), _ptr(positions), c_int(row0), c_int(n_rows), _ptr(tcgen05_error_flag(q.device)), _stream(), _ptr(sinks),
-        _ptr(slopes), _ptr(rates), c_int(v_heads), c_float(cap), c_int(keep))
+    fn = kernels().cbis_paged_prefill_tc5
+    if fn.argtypes is None:      # plain numbers are converted by their declared types: a third of the time that an object each takes
+        P, I = c_void_p, c_int
+        fn.argtypes = [P, I, I, P, P, I, P, I, P, P, P, I, I, I, I, I, I, I, I, c_float, I, I, I, P, P, I, I, P, P, P, P, P, I, c_float, I]
+    st = fn(q.data_ptr(), q.stride(0), q.shape[0], k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], block_table.data_ptr(),
+            block_table.shape[1], cu_rows.data_ptr(), seg_start.data_ptr(), out.data_ptr(), out.stride(0), seg0, n_seg, max_seg_rows, n_head,
+            n_kv_head, head_dim, page_size, scale, window, n_chunks, chunk_keys, _at(partial) or None, _at(positions) or None, row0, n_rows,
+            tcgen05_error_flag(q.device).data_ptr(), _stream(), _at(sinks) or None, _at(slopes) or None, _at(rates) or None, v_heads, cap, keep)
     _check(st, "paged_prefill_tc5", f"segments={n_seg} heads={n_head}/{n_kv_head} page={page_size} chunks={n_chunks}x{chunk_keys}")
 
 
