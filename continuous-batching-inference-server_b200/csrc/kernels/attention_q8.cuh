@@ -346,7 +346,7 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float s = q8_scale(top), inv = 1.f / s;
+        const float s = q8_scale(top), inv = q8_inverse(s);
         const size_t row = ((size_t)(slot / a.ps) * a.n_kv_head + p.hk) * a.ps + slot % a.ps;
         int8_t* dst = (warp ? a.vc : a.kc) + row * hd;
 #pragma unroll

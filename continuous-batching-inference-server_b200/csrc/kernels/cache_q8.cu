@@ -3,22 +3,24 @@
 //
 // Both are bound by their bytes once there are some megabytes of them, and by the launch below that.
 #include "cache_q8.cuh"
+#include "packed.cuh"
 #include <string.h>
 
 namespace cbis {
 
 // Rows with 16-byte loads: `lpr` lanes (a power of two) to a row, each with IT pieces of 16 bytes of it.  A row's largest magnitude
 // is found with shuffles inside its lanes while the numbers stay in registers, so the row is read once.
+// (More rows to a thread gained nothing: 2,048 tokens of 16 heads of 128 were 11.2 us with one, 11.4 with two and 12.0 with four.)
 template <typename TT, int IT>
 __global__ void __launch_bounds__(128)
 kv_write_q8_kernel(const TT* qkv, int ld, int k_off, int v_off, int8_t* kc, float* ks, int8_t* vc, float* vs, const int* slot_mapping,
-                   int n_slots, unsigned n_rows, int heads, int hd, int hd_v, int ps, int lpr_shift, int both) {
+                   int n_slots, unsigned n_rows, int heads, int hd, int hd_v, int ps, int ps_shift, int lpr_shift, int token_shift, int both) {
   constexpr int E = 16 / sizeof(TT);
   pdl_trigger();
   const int lpr = 1 << lpr_shift, sub = threadIdx.x & (lpr - 1);
   const unsigned unit = (blockIdx.x << (7 - lpr_shift)) + (threadIdx.x >> lpr_shift), per_token = heads << both;      // token, key or value, head
   const bool in_range = unit < n_rows;
-  const unsigned token = in_range ? unit / per_token : 0, place = in_range ? unit - token * per_token : 0;
+  const unsigned token = in_range ? (token_shift >= 0 ? unit >> token_shift : unit / per_token) : 0, place = in_range ? unit - token * per_token : 0;
   const bool which = place >= (unsigned)heads;
   const int h = which ? place - heads : place, width = which ? hd_v : hd;
   const TT* src = qkv + (size_t)token * ld + (which ? v_off : k_off) + h * width;
@@ -31,34 +33,40 @@ kv_write_q8_kernel(const TT* qkv, int ld, int k_off, int v_off, int8_t* kc, floa
     const int at = (i * lpr + sub) * E;
     raw[i] = in_range && at < width ? *reinterpret_cast<const uint4*>(src + at) : make_uint4(0, 0, 0, 0);
   }
-  float x[IT][E];
-  unsigned top = 0;
+  unsigned top = 0;      // bfloat16: the upper and the lower half of every word at once
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
     const unsigned w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (E == 8) {
-        x[i][2 * e] = __uint_as_float(w[e] << 16);
-        x[i][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-      } else {
-        x[i][e] = __uint_as_float(w[e]);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) top = max(top, q8_bits(x[i][e]));
+    for (int e = 0; e < 4; ++e) top = E == 8 ? __vmaxu2(top, w[e] & 0x7fff7fffu) : max(top, w[e] & 0x7fffffffu);
   }
-  for (int o = lpr / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int o = lpr / 2; o > 0; o >>= 1) {
+    const unsigned other = __shfl_xor_sync(0xffffffffu, top, o);
+    top = E == 8 ? __vmaxu2(top, other) : max(top, other);
+  }
   if (!live) return;
-  const float scale = q8_scale(top), inv = 1.f / scale;
-  const size_t row = ((size_t)(slot / ps) * heads + h) * ps + slot % ps;
+  if (E == 8) top = max(top & 0xffff0000u, top << 16);
+  const float scale = q8_scale(top), inv = q8_inverse(scale);
+  const int page = ps_shift >= 0 ? slot >> ps_shift : slot / ps;
+  const size_t row = ((size_t)page * heads + h) * ps + (slot - page * ps);
   int8_t* dst = (which ? vc : kc) + row * width;
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
     const int at = (i * lpr + sub) * E;
     if (at >= width) continue;
-    if constexpr (E == 8) *reinterpret_cast<uint2*>(dst + at) = make_uint2(q8_codes4(x[i], scale, inv), q8_codes4(x[i] + 4, scale, inv));
-    else *reinterpret_cast<unsigned*>(dst + at) = q8_codes4(x[i], scale, inv);
+    const unsigned w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    float x[E];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (E == 8) {
+        x[2 * e] = __uint_as_float(w[e] << 16);
+        x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+      } else {
+        x[e] = __uint_as_float(w[e]);
+      }
+    }
+    if constexpr (E == 8) *reinterpret_cast<uint2*>(dst + at) = make_uint2(q8_codes4(x, scale, inv), q8_codes4(x + 4, scale, inv));
+    else *reinterpret_cast<unsigned*>(dst + at) = q8_codes4(x, scale, inv);
   }
   if (sub == 0) (which ? vs : ks)[row] = scale;
 }
@@ -82,7 +90,7 @@ kv_write_q8_any_kernel(const TT* qkv, int ld, int k_off, int v_off, int8_t* kc, 
   for (int i = lane; i < width; i += 32) top = max(top, q8_bits(to_f32(src[i])));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float scale = q8_scale(top), inv = 1.f / scale;
+  const float scale = q8_scale(top), inv = q8_inverse(scale);
   const size_t row = ((size_t)(slot / ps) * heads + h) * ps + slot % ps;
   int8_t* dst = (which ? vc : kc) + row * width;
   for (int i = lane; i < width; i += 32) dst[i] = (int8_t)q8_code(to_f32(src[i]), scale, inv);
@@ -93,7 +101,9 @@ kv_write_q8_any_kernel(const TT* qkv, int ld, int k_off, int v_off, int8_t* kc, 
 __device__ __forceinline__ void q8_numbers(unsigned w, float* v) {
   w ^= 0x80808080u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650 | i)) - 8388736.f;
+  for (int i = 0; i < 4; i += 2)
+    unpack2(add2(pack2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650 | i)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7651 | i))),
+                 pack2(-8388736.f, -8388736.f)), v[i], v[i + 1]);
 }
 
 // grid (pages of a request that may be read, requests, parts of a page): a block takes a part of the rows (head, token) of one page of
@@ -129,6 +139,35 @@ kv_read_q8_kernel(const int8_t* kc, const float* ks, const int8_t* vc, const flo
     const int8_t* src = (which ? vc : kc) + row0 * width;
     const float* scales = (which ? vs : ks) + row0;
     TT* dst = (which ? vo : ko) + row0 * width;
+    if (N > 1 && n == ps && (first <= j0 || kept >= j0 + ps) && width == N << lpr_shift) {
+      // a whole page of rows of a power of two of pieces: one run of codes, four pieces of it on their way to a thread
+      const int units = rows << lpr_shift;
+      for (int u0 = blockIdx.z * 1024 + threadIdx.x; u0 < units; u0 += gridDim.z * 1024) {
+        float scale[4];
+        uint2 raw[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int u = min(u0 + k * 256, units - 1);
+          scale[k] = scales[u >> lpr_shift];
+          if constexpr (N == 8) raw[k] = reinterpret_cast<const uint2*>(src)[u];
+          else raw[k].x = reinterpret_cast<const unsigned*>(src)[u];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (u0 + k * 256 >= units) break;
+          float v[8];
+          q8_numbers(raw[k].x, v);
+          if constexpr (N == 8) q8_numbers(raw[k].y, v + 4);
+          const unsigned long long s2 = pack2(scale[k], scale[k]);
+#pragma unroll
+          for (int e = 0; e < N; e += 2) unpack2(mul2(pack2(v[e], v[e + 1]), s2), v[e], v[e + 1]);
+          TT* p = dst + (size_t)(u0 + k * 256) * N;
+          if constexpr (N == 8) store8(p, v);
+          else *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+      }
+      continue;
+    }
     for (int r0 = blockIdx.z * (256 >> lpr_shift) + (threadIdx.x >> lpr_shift); r0 < rows; r0 += 4 * step) {
       int at[4];
 #pragma unroll
@@ -204,9 +243,15 @@ CBIS_EXPORT int cbis_kv_write_q8(const void* call) {
   const int its = (widest + lpr * E - 1) / (lpr * E);
   const long long blocks = vec ? (n_rows + 128 / lpr - 1) / (128 / lpr) : (n_rows + 3) / 4;
   if (n_rows > 0x7fffffffLL || blocks > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
+  int token_shift = -1, ps_shift = -1;
+  for (int i = 0; i < 31; ++i) {
+    if (heads << both == 1 << i) token_shift = i;
+    if (ps == 1 << i) ps_shift = i;
+  }
 #define CBIS_WRITE(TT, IT)                                                                                                        \
   return (int)launch_pdl(kv_write_q8_kernel<TT, IT>, dim3((unsigned)blocks), dim3(128), 0, st, (const TT*)qkv, ld, k_off, v_off,  \
-                         (int8_t*)kc, (float*)ks, (int8_t*)vc, (float*)vs, slot_mapping, n_slots, (unsigned)n_rows, heads, hd, hd_v, ps, shift, both)
+                         (int8_t*)kc, (float*)ks, (int8_t*)vc, (float*)vs, slot_mapping, n_slots, (unsigned)n_rows, heads, hd,    \
+                         hd_v, ps, ps_shift, shift, token_shift, both)
 #define CBIS_WRITE_ANY(TT)                                                                                                        \
   return (int)launch_pdl(kv_write_q8_any_kernel<TT>, dim3((unsigned)blocks), dim3(128), 0, st, (const TT*)qkv, ld, k_off, v_off,  \
                          (int8_t*)kc, (float*)ks, (int8_t*)vc, (float*)vs, slot_mapping, n_slots, n_rows, heads, hd, hd_v, ps, both)
@@ -259,9 +304,10 @@ CBIS_EXPORT int cbis_kv_read_q8(const void* call) {
   int shift = 0;
   const int widest = vc && hd_v > hd ? hd_v : hd;
   while (shift < 5 && (vec ? N : 1) << shift < widest) ++shift;
-  // parts of a page: four rows to a thread if there are blocks enough, fewer rows for a few pages
+  // parts of a page: eight rows to a thread if there are blocks enough (23 requests of 90 to 1,100 tokens, 25 heads of 64: 28.2 us with
+  // four, 26.0 so), fewer rows for a few pages
   const long long rows = (long long)heads * ps, per_block = 256 >> shift, pages = blocks * n_seg;
-  long long parts = (rows + 4 * per_block - 1) / (4 * per_block), finest = (rows + per_block - 1) / per_block;
+  long long parts = (rows + 8 * per_block - 1) / (8 * per_block), finest = (rows + per_block - 1) / per_block;
   if (pages * parts < 4 * 148) parts = (4 * 148 + pages - 1) / pages;
   if (parts > finest) parts = finest;
   if (parts > 65535) parts = 65535;

@@ -6,6 +6,7 @@
 // 2^-121 are read back as 0.
 #pragma once
 #include "common.cuh"
+#include "packed.cuh"
 
 namespace cbis {
 
@@ -14,23 +15,30 @@ constexpr float Q8_FLOOR = 7.52316384526264e-37f;      // 2^-120
 // The largest magnitude as the bits of |x|: ordered like the magnitudes, an infinity above every number and a NaN above that.
 __device__ __forceinline__ unsigned q8_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// amax / 127 rounded to nearest: the product with 1 / 127 and what it leaves over, times 1 / 127 again (Markstein's correction of a
+// quotient: with a correctly rounded reciprocal the second sum is the correctly rounded quotient).
 __device__ __forceinline__ float q8_scale(unsigned amax_bits) {
-  return amax_bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__fdiv_rn(__uint_as_float(amax_bits), 127.f), Q8_FLOOR);
+  const float a = __uint_as_float(amax_bits), c = 1.f / 127.f, q = a * c;
+  return amax_bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(fmaf(fmaf(-q, 127.f, a), c, q), Q8_FLOOR);
 }
+// 1 / scale to 2^-22 or so: the exact way below needs no more.
+__device__ __forceinline__ float q8_inverse(float scale) { return __frcp_rn(scale); }
 
 // The codes of four numbers, a byte each.  Adding 1.5 * 2^23 rounds x / scale to a whole number, ties to even, and leaves it in the low
 // bits; the quotient is a product with the reciprocal, good to 2^-22, so only a number that close to a half step needs the exact way.
 __device__ __forceinline__ int q8_code(float x, float scale, float inv);
 __device__ __forceinline__ unsigned q8_codes4(const float* x, float scale, float inv) {
-  float f[4];
-  bool close = false;
+  float f[4], far = 0.f;
+  const unsigned long long inv2 = pack2(inv, inv), up = pack2(12582912.f, 12582912.f), down = pack2(-12582912.f, -12582912.f), neg = pack2(-1.f, -1.f);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float y = x[i] * inv;
-    f[i] = y + 12582912.f;
-    close |= fabsf(y - (f[i] - 12582912.f)) > 0.4999f;
+  for (int i = 0; i < 4; i += 2) {
+    const unsigned long long y = mul2(pack2(x[i], x[i + 1]), inv2), z = add2(y, up);
+    float d0, d1;
+    unpack2(z, f[i], f[i + 1]);
+    unpack2(fma2(add2(z, down), neg, y), d0, d1);
+    far = fmaxf(far, fmaxf(fabsf(d0), fabsf(d1)));
   }
-  if (close) {
+  if (far > 0.4999f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = (float)q8_code(x[i], scale, inv) + 12582912.f;
   }
