@@ -15,8 +15,9 @@ from typing import Dict, List, Optional, Sequence
 
 import torch
 
+from ..kernels import ops
 from ..kernels.library import host
-from ..parts import CacheNeed
+from ..parts import AttentionLike, CacheNeed
 
 
 @dataclass
@@ -26,6 +27,12 @@ class LayerCache:
     arrays: Dict[str, torch.Tensor]
     page_size: int
     window: int
+    scales: Optional[Dict[str, torch.Tensor]] = None      # an 8-bit cache: the arrays hold codes, and these ``[num_pages, heads, page_size]`` their scales
+    values: Optional["LayerCache"] = None                 # an 8-bit cache: the pages that the codes are read back into (shared by all layers)
+
+    def coded(self, name: str) -> ops.Q8Pages:
+        """The codes and scales of an array of an 8-bit cache."""
+        return ops.Q8Pages(self.arrays[name], self.scales[name])
 
     @property
     def k(self) -> torch.Tensor:
@@ -43,9 +50,13 @@ class CacheGroup:
     page_size: int
     num_pages: int
     storage: Optional[torch.Tensor] = None   # one flat allocation: [layer][array][page][head][token][width]
+    scale_storage: Optional[torch.Tensor] = None      # of an 8-bit cache: [layer][array][page][head][token]
 
-    def bytes_per_page(self, itemsize: int) -> int:
-        return len(self.layers) * self.need.elements_per_token() * self.page_size * itemsize
+    def bytes_per_page(self, itemsize: int, coded: bool = False) -> int:
+        """Bytes of a page in all layers of the group; ``coded``: a byte an element and 4 a token and head, instead of ``itemsize``."""
+        per_token = self.need.elements_per_token()
+        per_token = per_token + 4 * sum(a.heads for a in self.need.arrays) if coded else per_token * itemsize
+        return len(self.layers) * per_token * self.page_size
 
 
 def _need_with_readers(model, li: int, need: CacheNeed) -> CacheNeed:
@@ -75,11 +86,36 @@ def cache_groups_of(model, page_size: int) -> List[CacheGroup]:
     return groups
 
 
+CACHE_DTYPES = (None, "int8")
+
+
+def refuse_coded(model) -> None:
+    """Raises if a mixer keeps or reads a cache otherwise than through the step's attention (``StepContext.attention``), which is what
+    reads and writes an 8-bit cache."""
+    for li, layer in enumerate(model.layers):
+        need = layer.mixer.cache_need()
+        if need is None and layer.spec.cache_source is None:
+            continue
+        for m in layer.mixer.cache_users():
+            names = set(getattr(m, "kv_arrays", ("k", "v")))
+            if not isinstance(m, AttentionLike) or (need is not None and {a.name for a in need.arrays} != names):
+                raise ValueError(f"layer {li}: {type(m).__name__} does not keep keys and values that the attention kernels read; "
+                                 f"its cache cannot be kept in 8 bits")
+
+
 class CachePool:
     def __init__(self, model, *, page_size: int = 16, num_pages: Optional[int] = None, max_requests: int = 16,
-                 max_tokens: Optional[int] = None, memory_fraction: float = 0.85, device="cuda"):
+                 max_tokens: Optional[int] = None, memory_fraction: float = 0.85, device="cuda", cache_dtype: Optional[str] = None):
         """``num_pages`` per group, or ``max_tokens`` (pages = ceil(max_tokens / page_size)), or what
-        ``memory_fraction`` of the free device memory holds."""
+        ``memory_fraction`` of the free device memory holds.  ``cache_dtype`` "int8": keys and values are kept as 8-bit codes
+        with a scale per token and head (``kernels.ops.Q8Pages``) instead of in the model's type; beside them the pool
+        then holds the pages of one layer in that type, into which codes are read back."""
+        if cache_dtype not in CACHE_DTYPES:
+            raise ValueError(f"cache_dtype {cache_dtype!r} is not one of {list(CACHE_DTYPES)}")
+        self.cache_dtype = cache_dtype
+        coded = cache_dtype == "int8"
+        if coded:
+            refuse_coded(model)
         if page_size <= 0:
             raise ValueError("page_size must be positive")
         self.model, self.page_size, self.max_requests = model, page_size, max_requests
@@ -90,26 +126,37 @@ class CachePool:
             num_pages = -(-max_tokens // page_size)
         if num_pages is None:
             free, _ = torch.cuda.mem_get_info(self.device)
-            per_page = sum(g.bytes_per_page(itemsize) for g in self.groups) or 1
+            per_page = sum(g.bytes_per_page(itemsize, coded) for g in self.groups) or 1
+            if coded:
+                per_page += max((g.need.elements_per_token() for g in self.groups), default=0) * page_size * itemsize
             num_pages = max(1, int(free * memory_fraction) // per_page)
             # no request can use more than max_requests * max_positions tokens
             num_pages = min(num_pages, max_requests * (-(-model.spec.max_positions // page_size)))
         self.layer_cache: Dict[int, LayerCache] = {}
         specs = []
-        align = 256 // itemsize                      # every array starts on a 256-byte boundary (TMA wants 16)
+        align = 256 // (1 if coded else itemsize)    # every array starts on a 256-byte boundary (TMA wants 16)
         for gi, g in enumerate(self.groups):
             g.num_pages = int(num_pages)
             sizes = [(-(-g.num_pages * a.heads * page_size * a.width // align) * align) for a in g.need.arrays]
-            g.storage = torch.zeros(len(g.layers) * sum(sizes), dtype=self.dtype, device=self.device)
-            at = 0
+            g.storage = torch.zeros(len(g.layers) * sum(sizes), dtype=torch.int8 if coded else self.dtype, device=self.device)
+            rows = [g.num_pages * a.heads * page_size for a in g.need.arrays]
+            if coded:
+                g.scale_storage = torch.zeros(len(g.layers) * sum(rows), dtype=torch.float32, device=self.device)
+            at = at_scale = 0
             for li in g.layers:
-                arrays = {}
+                arrays, scales = {}, {}
                 for a, size in zip(g.need.arrays, sizes):
                     n = g.num_pages * a.heads * page_size * a.width
                     arrays[a.name] = g.storage[at:at + n].view(g.num_pages, a.heads, page_size, a.width)
                     at += size
-                self.layer_cache[li] = LayerCache(gi, arrays, page_size, g.need.window)
+                    if coded:
+                        n = g.num_pages * a.heads * page_size
+                        scales[a.name] = g.scale_storage[at_scale:at_scale + n].view(g.num_pages, a.heads, page_size)
+                        at_scale += n
+                self.layer_cache[li] = LayerCache(gi, arrays, page_size, g.need.window, scales if coded else None)
             specs.append(host().GroupSpec(page_size, g.num_pages, g.need.window, g.need.keep_first))
+        if coded:
+            self._read_back_pages(itemsize)
         if not specs:  # a model without any cache still needs request slots and lengths: pages that are counted only
             specs.append(host().GroupSpec(page_size, int(num_pages), 0))
         for li, layer in enumerate(model.layers):
@@ -126,6 +173,21 @@ class CachePool:
             if need is not None:
                 self.state[li] = torch.zeros((max_requests, *need.shape), dtype=need.dtype, device=self.device)
 
+    def _read_back_pages(self, itemsize: int) -> None:
+        """One layer's pages in the model's type, page p of which takes what is read back of page p of any layer."""
+        align = 256 // itemsize
+        sizes = {gi: [(-(-g.num_pages * a.heads * self.page_size * a.width // align) * align) for a in g.need.arrays] for gi, g in enumerate(self.groups)}
+        self.read_back = torch.zeros(max((sum(v) for v in sizes.values()), default=0), dtype=self.dtype, device=self.device)
+        for gi, g in enumerate(self.groups):
+            arrays, at = {}, 0
+            for a, size in zip(g.need.arrays, sizes[gi]):
+                n = g.num_pages * a.heads * self.page_size * a.width
+                arrays[a.name] = self.read_back[at:at + n].view(g.num_pages, a.heads, self.page_size, a.width)
+                at += size
+            values = LayerCache(gi, arrays, self.page_size, g.need.window)
+            for li in g.layers:
+                self.layer_cache[li].values = values
+
     def max_blocks(self, gi: int) -> int:
         return -(-self.model.spec.max_positions // self.page_size)
 
@@ -135,7 +197,7 @@ class CachePool:
 
     def bytes_per_token(self) -> int:
         itemsize = torch.empty((), dtype=self.dtype).element_size()
-        return sum(len(g.layers) * g.need.elements_per_token() * itemsize for g in self.groups)
+        return sum(g.bytes_per_page(itemsize, self.cache_dtype == "int8") // g.page_size for g in self.groups)
 
     def poison_pages(self, group: int, pages: Sequence[int]) -> None:
         """Fills the given pages of every array of every layer of ``group`` with NaN (a debugging aid: a
@@ -145,5 +207,6 @@ class CachePool:
             return
         idx = torch.tensor(sorted(set(int(p) for p in pages)), dtype=torch.long, device=self.device)
         for li in self.groups[group].layers:
-            for t in self.layer_cache[li].arrays.values():
+            lc = self.layer_cache[li]
+            for t in (lc.scales or lc.arrays).values():      # codes are always numbers: with a scale of NaN none of them is
                 t.index_fill_(0, idx, float("nan"))

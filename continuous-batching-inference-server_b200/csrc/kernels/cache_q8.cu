@@ -114,8 +114,7 @@ __global__ void __launch_bounds__(256)
 kv_read_q8_kernel(const int8_t* kc, const float* ks, const int8_t* vc, const float* vs, TT* ko, TT* vo, const int* block_table, int max_blocks,
                   int num_pages, const int* seg_start, const int* seg_ctx, int heads, int hd, int hd_v, int ps, int window, int keep,
                   int kept_blocks, int whole, int lpr_shift) {
-  pdl_trigger();
-  pdl_wait();
+  pdl_wait();      // no early start for the kernel behind: those that read pages ask for the first of them before they wait
   const int s = blockIdx.y, ctx = min(seg_ctx[s], max_blocks * ps);
   if (ctx <= 0) return;
   int first = first_seen(min(max(seg_start[s], 0), ctx - 1), window), kept = kept_end(ctx - 1, window, keep);

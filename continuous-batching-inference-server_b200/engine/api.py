@@ -38,7 +38,7 @@ class Engine:
                  num_pages: Optional[int] = None, max_tokens: Optional[int] = None, max_num_seqs: int = 16,
                  max_batched_tokens: int = 512, prefill_chunk: Optional[int] = None,
                  memory_fraction: float = 0.85, device: str = "cuda", poison_freed_pages: Optional[bool] = None,
-                 max_model_len: Optional[int] = None):
+                 max_model_len: Optional[int] = None, cache_dtype: Optional[str] = None):
         """``model``: a folder with config.json and model.safetensors, or a loaded ``Model``.
         Engine options in the reference's terms: ``page_size`` = kPageSize (include/config.hpp:20),
         ``num_pages`` = kMaxPages, ``max_num_seqs`` = kMaxSlots, ``max_batched_tokens`` =
@@ -49,7 +49,9 @@ class Engine:
         token slot beyond a request's length in a page that was used before, shows as NaN logits.
         ``max_model_len``: the longest request the engine takes (block tables are sized for it); at most the model's
         own position limit; for a model without one the default is what the pool is asked to hold (``num_pages`` or
-        ``max_tokens``), else 32,768."""
+        ``max_tokens``), else 32,768.  ``cache_dtype`` "int8" keeps keys and values in 8 bits, with a scale per token and head: about half
+        the bytes per token of a bfloat16 cache, a quarter of a 32-bit one's.  Every query, a prompt's own too, sees the keys and
+        values as they are kept, so the logits do not depend on how a prompt is cut."""
         if not torch.cuda.is_available():
             raise RuntimeError("the engine needs a CUDA device (sm_100a); there is no CPU path")
         self.model = load_model(model, dtype, device) if isinstance(model, str) else model
@@ -62,7 +64,7 @@ class Engine:
         elif max_model_len is not None and int(max_model_len) < own_limit:
             self.model.spec = dataclasses.replace(self.model.spec, max_positions=int(max_model_len))
         self.pool = CachePool(self.model, page_size=page_size, num_pages=num_pages, max_tokens=max_tokens,
-                              max_requests=max_num_seqs, memory_fraction=memory_fraction, device=device)
+                              max_requests=max_num_seqs, memory_fraction=memory_fraction, device=device, cache_dtype=cache_dtype)
         self.runner = ModelRunner(self.model, self.pool, max_batched_tokens=max_batched_tokens,
                                   max_num_seqs=max_num_seqs)
         self.limits = dict(max_num_seqs=max_num_seqs, max_batched_tokens=max_batched_tokens,

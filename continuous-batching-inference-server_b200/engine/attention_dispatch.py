@@ -13,7 +13,9 @@ positions, counted from position 0: the query sees its own block's keys up to p)
   CBIS_TCGEN05=0): the tiled mma.sync kernel;
 * 32-bit, head size in steps of 16 up to 128, longer segments: the tiled 32-bit kernel (decoding rows: the general
   kernel);
-* everything else: the general kernel, after the cache-write kernel.
+* everything else: the general kernel, after the cache-write kernel;
+* a cache in 8 bits: its own kernels for decoding rows and for longer segments (``_coded``), or, for what they do not take, the kernels
+  above over the values read back.
 
 A mixer may also name (attributes, all optional): ``v_head_dim`` (values of another width than the keys; with one
 cached array for keys and values the values are the first entries of its rows), ``slopes`` (a distance bias per
@@ -150,9 +152,68 @@ def _mixed(ctx, mixer, qkv, cache, view, out, gate) -> int:
     return vd
 
 
+class _Reader:
+    """A mixer whose keys and values have been stored already."""
+
+    def __init__(self, mixer):
+        self._mixer, self.own_kv = mixer, False
+
+    def __getattr__(self, name):
+        return getattr(self._mixer, name)
+
+
+def _coded(ctx, mixer, qkv, cache, view, out, gate) -> int:
+    """Attention over an 8-bit cache.  Keys and values of one width, a multiple of 16 up to 256, in two arrays: the decoding rows through the
+    kernel that stores the current token itself, the longer segments, after the cache-write kernel, through ``paged_prefill_q8``.
+    For anything else (other widths, one array for both, weights mixed across heads) this step's keys and values are stored, what the
+    rows see is read back, and the kernels over values do the rest."""
+    T, nd, hd, ps, H, G = ctx.n_rows, ctx.n_decode, mixer.head_dim, cache.page_size, mixer.n_head, mixer.n_kv_head
+    k_name, v_name = getattr(mixer, "kv_arrays", ("k", "v"))
+    one = k_name == v_name
+    vd = int(getattr(mixer, "v_head_dim", 0) or hd)
+    k_off = mixer.d_q
+    v_off = k_off if one else k_off + mixer.d_kv
+    k, v = cache.coded(k_name), None if one else cache.coded(v_name)
+    per = 8 if qkv.dtype == torch.bfloat16 else 4
+    extra = {n: getattr(mixer, n, None) for n in ("slopes", "sinks", "q_temp", "rates")}
+    extra.update(cap=float(getattr(mixer, "cap", 0.0)), keep=int(getattr(mixer, "keep_first", 0)))
+    if (not one and getattr(mixer, "talk", None) is None and ops.attention_q8_takes(hd, vd) and qkv.stride(0) % per == 0
+            and qkv.data_ptr() % 16 == 0 and nd <= ops.ATTENTION_Q8_MAX_ROWS
+            and (T == nd or ops.prefill_q8_takes(ctx.n_segments - nd, ctx.max_seg_rows, H, G, hd, ps, qkv.dtype, **extra))):
+        work, limit = (cache.values.arrays[k_name], cache.values.arrays[v_name]), ctx.ctx_limit
+        if nd > 0:
+            scratch = ctx.decode_scratch(*_coded_scratch(ctx, nd, 1, nd, H, G, hd, limit, qkv.dtype))
+            ops.paged_decode_q8(qkv[:nd], k_off if mixer.own_kv else -1, v_off if mixer.own_kv else -1, k, v, view.block_table, ctx.row_seq,
+                                ctx.positions, view.slot_mapping, out[:nd], *scratch, H, G, hd, ps, mixer.scale, mixer.window, limit, **extra)
+        if T > nd:
+            n = ctx.n_segments - nd
+            if mixer.own_kv:
+                ops.kv_write_q8(qkv[nd:], k_off, v_off, k, v, view.slot_mapping[nd:], G, hd, ps)
+            scratch = ctx.decode_scratch(*_coded_scratch(ctx, T - nd, ctx.max_seg_rows, n, H, G, hd, limit, qkv.dtype))
+            ops.paged_prefill_q8(qkv, k, v, view.block_table, ctx.cu_rows, ctx.seg_start, ctx.seg_ctx, ctx.positions, out, nd, n, nd, T - nd,
+                                 ctx.max_seg_rows, H, G, hd, ps, mixer.scale, mixer.window, limit, *scratch, work, **extra)
+        return hd
+    if mixer.own_kv:
+        ops.kv_write_q8(qkv, k_off, v_off, k, v, view.slot_mapping, G, hd, ps, v_head_dim=vd)
+    window, rows, keep = mixer.window, max(ctx.max_seg_rows, 1), extra["keep"]
+    tokens = min(ctx.ctx_limit, abs(window) + rows) if window else ctx.ctx_limit
+    ops.kv_read_q8(k, v, cache.values.arrays[k_name], None if one else cache.values.arrays[v_name], view.block_table, ctx.seg_start,
+                   ctx.seg_ctx, tokens, window, keep, whole_pages=True)
+    return run_attention(ctx, _Reader(mixer), qkv, cache.values, view, out, gate)
+
+
+def _coded_scratch(ctx, rows, most, n_seg, n_head, n_kv_head, hd, limit, dtype):
+    key = ("coded_scratch", rows, most, n_seg, n_head, n_kv_head, hd)
+    if key not in ctx.shared:
+        ctx.shared[key] = ops.attention_q8_scratch(rows, most, n_seg, n_head, n_kv_head, hd, limit, dtype)
+    return ctx.shared[key]
+
+
 def run_attention(ctx, mixer, qkv, cache, view, out, gate=None) -> int:
     nd = ctx.n_decode
     T = ctx.n_rows
+    if cache.scales is not None:
+        return _coded(ctx, mixer, qkv, cache, view, out, gate)
     if getattr(mixer, "talk", None) is not None:
         return _mixed(ctx, mixer, qkv, cache, view, out, gate)
     hd, ps = mixer.head_dim, cache.page_size

@@ -714,6 +714,7 @@ def _kv_read_q8(kc, ks, vc, vs, k_out, v_out, table: int, blocks: int, start: in
 
 
 ATTENTION_Q8_MAX_HEAD_DIM = 256
+ATTENTION_Q8_MAX_ROWS = 4096        # decoding rows, or row tiles of chunks, of one launch
 
 
 def attention_q8_takes(head_dim: int, v_head_dim: int = 0) -> bool:
@@ -847,6 +848,12 @@ def prefill_q8_reads_back(max_seg_rows: int, n_head: int, n_kv_head: int, head_d
     if dtype == torch.float32:
         return slopes is None and sinks is None and q_temp is None and not cap and not keep
     return True
+
+
+def prefill_q8_takes(n_seg: int, max_seg_rows: int, n_head: int, n_kv_head: int, head_dim: int, page_size: int, dtype, **extra) -> bool:
+    """Whether ``paged_prefill_q8`` with ``work`` takes these sizes (the kernel that reads codes counts its row tiles)."""
+    return (prefill_q8_reads_back(max_seg_rows, n_head, n_kv_head, head_dim, page_size, dtype, **extra)
+            or _q8_scratch(n_seg, max_seg_rows, n_head, n_kv_head, head_dim, dtype_code(dtype), 1)[0] == 0)
 
 
 def paged_prefill_q8(q, k_pages, v_pages, block_table, cu_rows, seg_start, seg_ctx, positions, out, seg0, n_seg, row0, n_rows, max_seg_rows,

@@ -136,6 +136,10 @@ class Mixer(Part):
     def state_need(self) -> Optional[StateNeed]:
         return None
 
+    def cache_users(self) -> List["Mixer"]:
+        """The mixers that read and write the layer's cache: this one, or those that it is put together from."""
+        return [self]
+
     def forward(self, ctx, h: torch.Tensor, cache, state: Optional[torch.Tensor]) -> Delta:
         """``cache``: the ``LayerCache`` of this layer (or of the layer it reads), None if it keeps none;
         ``cache.arrays[name]`` are its pages ``[num_pages, heads, page_size, width]``, addressed through

@@ -67,7 +67,7 @@ class PreNormBlock(Block):
         a, f, n1, n2 = self.mixer, self.feed_forward, self.norm_mixer, self.norm_feed_forward
         key = None
         if (type(a) is PagedAttention and type(f) is DenseFeedForward and type(n1) is LayerNorm and type(n2) is LayerNorm
-                and a.own_kv and a.head_dim in (64, 128) and cache is not None and cache.page_size % 16 == 0
+                and a.own_kv and a.head_dim in (64, 128) and cache is not None and not cache.scales and cache.page_size % 16 == 0
                 and a.width == f.width == n1.width == n2.width and a.width % 8 == 0 and f.inner % 8 == 0
                 and a.w_qkv is not None and a.w_qkv.is_cuda and a.w_qkv.dtype == torch.bfloat16):
             key = ("decode_layers", a.width, a.n_head, a.n_kv_head, a.head_dim, f.inner, f.activation, a.window, a.scale,

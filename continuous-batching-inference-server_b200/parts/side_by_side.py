@@ -49,6 +49,9 @@ class SideBySide(Mixer):
     def state_need(self):
         return self.left.state_need() or self.right.state_need()
 
+    def cache_users(self):
+        return [m for m in (self.left, self.right) if m.cache_need() is not None]
+
     def tensors(self, prefix):
         return self.left.tensors(prefix + self.names[0]) + self.right.tensors(prefix + self.names[1])
 
