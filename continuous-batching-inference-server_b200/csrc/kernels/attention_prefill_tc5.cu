@@ -36,11 +36,18 @@
 // and keys with a cap a few times their largest score always are: six multiply-adds a score, where an exponential and a
 // quotient would triple the load of the special-function units), else it goes through an exponential.
 //
+// CODED: keys and values are whole numbers (the codes of an 8-bit cache, exact in bfloat16) with a scale per key and one per value:
+// the scores are multiplied by the one and the weights, on their way to bfloat16, by the other, so nothing is rounded more often than
+// over keys and values in bfloat16.  The softmax threads bring a tile's 128 scales through the table's place in shared memory,
+// asked for a tile ahead.  A value whose scale is not finite makes its key's scores not-a-number (its rows' results then are, and a row
+// that does not see it multiplies by zero).
+//
 // Every wait on an mbarrier is bounded; when a limit runs out the block sets *error, stops, frees its
 // tensor memory and returns (its output rows are then invalid, and the host raises).
 #include "attention_merge.cuh"
 #include "packed.cuh"
 
+#include <atomic>
 #include <cuda.h>
 #include <math.h>
 #include <mutex>
@@ -203,14 +210,15 @@ __device__ __forceinline__ void softmax_warps_meet() {
 // and at the end each hands sum, reference and one half of the head dims to the other through distributed shared memory
 // and finishes the other half.
 // The row tile with the most keys decides how long the kernel runs, and its chain of tiles is halved this way.
-template <int HD, bool BIAS, bool EXT>
+template <int HD, bool BIAS, bool EXT, bool CODED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 2)
 paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const int* block_table, int max_blocks,
                          const int* cu_rows, const int* seg_start, __nv_bfloat16* out, int out_ld, int seg0, int n_seg,
                          int n_head, int n_kv_head, int ps, float scale_log2e, int window, int n_chunks, int chunk_keys,
                          float* partial, int row0, int* error, const float* __restrict__ sinks,
-                         const float* __restrict__ slopes, const float* __restrict__ rates, int v_heads, float cap, int keep) {
+                         const float* __restrict__ slopes, const float* __restrict__ rates, int v_heads, float cap, int keep,
+                         const float* k_scales, const float* v_scales) {
   constexpr int PBUF = p_buffers(HD), HALVES = HD / 64, Q_BYTES = HALVES * Q_HALF_BYTES, KV_BYTES = HALVES * KV_HALF_BYTES;
   extern __shared__ __align__(1024) unsigned char base[];   // no byte to spare for rounding the address up: checked below
   unsigned char* sQ = base;                                   // 2 halves of the head dim
@@ -435,14 +443,36 @@ paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // exponentials and eight 16-byte stores of P: no exchange between threads anywhere.
     const int p = pos0 + r;                         // this row's position
     // a row that gives up leaves the loop, or, where the warps meet in every tile, goes on to the next meeting
-#define TC5_STOP { if constexpr (BIAS) continue; else break; }
+#define TC5_STOP { if constexpr (BIAS || CODED) continue; else break; }
     float slope2 = 0.f, rate = 0.f;
     if constexpr (BIAS) {
       slope2 = slopes[h];                           // slope * ln(x) in log2 units is slope * log2(x)
       rate = rates[h];
     }
+    // CODED: the scales of column r of tile j (threads of the first 64 rows); columns behind the last key repeat it, and are masked
+    float k_scale = 0.f, v_scale = 0.f;
+    auto find_scales = [&](int j) {
+      if (r < BN && j < n_tiles) {
+        const int at = max(min(tile_at(j) * BN + r, (EXT ? max(kend, kept_upto) : kend) - 1), 0);
+        const size_t row = (size_t)max(bt[at / ps], 0) * n_kv_head * ps + at % ps;
+        k_scale = k_scales[row + hp.key * ps];
+        v_scale = v_scales[row + hp.value * ps];
+      }
+    };
+    if constexpr (CODED) find_scales(0);
     for (int j = 0; j < n_tiles; ++j) {
       const int j0 = tile_at(j) * BN;
+      if constexpr (CODED) {
+        softmax_warps_meet();
+        if (r < BN) {
+          const bool fine = fabsf(v_scale) < INFINITY;
+          table[r] = fine ? k_scale * scale_log2e : __uint_as_float(0x7fc00000u);
+          table[BN + r] = fine ? v_scale : 0.f;
+        }
+        softmax_warps_meet();
+        find_scales(j + 1);
+        if (!ok) continue;
+      }
       if constexpr (BIAS) {
         // the four warps meet before the table is overwritten and when it is done; a row that has given up goes on
         // meeting the others
@@ -461,9 +491,18 @@ paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
         for (int i = 0; i < BN; ++i) v[i] = fmaf(v[i], scale_log2e, -table[r + BN - 1 - i]);
       }
+      if constexpr (CODED) {     // from here on v is in log2 units
+#pragma unroll
+        for (int i = 0; i < BN; i += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(table + i);
+          unpack2(mul2(pack2(v[i], v[i + 1]), pack2(x.x, x.y)), v[i], v[i + 1]);
+          unpack2(mul2(pack2(v[i + 2], v[i + 3]), pack2(x.z, x.w)), v[i + 2], v[i + 3]);
+        }
+      }
       if constexpr (EXT) {       // from here on v is in log2 units, capped
+        const float unit = CODED ? 1.f : scale_log2e;
         if (cap > 0.f) {
-          const float to_x = scale_log2e * 0.6931471805599453f / cap, cap2 = cap * 1.4426950408889634f;
+          const float to_x = unit * 0.6931471805599453f / cap, cap2 = cap * 1.4426950408889634f;
           float big0 = 0.f, big1 = 0.f;
 #pragma unroll
           for (int i = 0; i < BN; i += 2) {
@@ -480,7 +519,7 @@ paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < BN; ++i) v[i] *= scale_log2e;
+          for (int i = 0; i < BN; ++i) v[i] *= unit;
         }
       }
       const bool edge = (j0 + BN - 1 > pos0) || (window != 0 && j0 < first_seen(pos0 + BM - 1, window)) || j0 + BN > kend;
@@ -512,7 +551,7 @@ paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
       mx0 = max3(mx0, v[BN - 4], v[BN - 3]);
       mx1 = max3(mx1, v[BN - 2], v[BN - 1]);
-      const float m_tile = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * (BIAS || EXT ? 1.f : scale_log2e);
+      const float m_tile = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * (BIAS || EXT || CODED ? 1.f : scale_log2e);
       const bool raise = m_tile > m + RAISE_BY || (m == -INFINITY && m_tile > m);
       if (j > 0 && __any_sync(0xffffffffu, raise)) {
         // rescale the row of O in tensor memory, which the products of the tile before write; rows that keep their reference multiply by 1
@@ -541,10 +580,14 @@ paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         for (int i = 0; i < 4; ++i) {
           const unsigned long long x = pack2(v[q8 * 8 + 2 * i], v[q8 * 8 + 2 * i + 1]);
           float e0, e1;
-          unpack2(BIAS || EXT ? add2(x, ref2) : fma2(x, scale2, ref2), e0, e1);
+          unpack2(BIAS || EXT || CODED ? add2(x, ref2) : fma2(x, scale2, ref2), e0, e1);
           e0 = ex2(e0);
           e1 = ex2(e1);
           psum = add2(psum, pack2(e0, e1));
+          if constexpr (CODED) {
+            const float2 x2 = *reinterpret_cast<const float2*>(table + BN + q8 * 8 + 2 * i);
+            unpack2(mul2(pack2(e0, e1), pack2(x2.x, x2.y)), e0, e1);
+          }
           __nv_bfloat162 b2 = __floats2bfloat162_rn(e0, e1);
           pk[q8][i] = *reinterpret_cast<unsigned*>(&b2);
         }
@@ -765,7 +808,8 @@ CBIS_EXPORT int cbis_paged_prefill_tc5(const void* q, int q_ld, int total_rows, 
                                        int max_seg_rows, int n_head, int n_kv_head, int hd, int ps, float scale,
                                        int window, int n_chunks, int chunk_keys, float* partial, const int* positions,
                                        int row0, int n_rows, int* error, void* stream, const float* sinks,
-                                       const float* slopes, const float* rates, int v_heads, float cap, int keep) {
+                                       const float* slopes, const float* rates, int v_heads, float cap, int keep,
+                                       const float* k_scales, const float* v_scales) {
   if (n_seg <= 0 || max_seg_rows <= 0) return CBIS_OK;
   if (n_chunks < 1 || (n_chunks > 1 && (chunk_keys <= 0 || chunk_keys % tc5::BN || !partial || !positions || n_rows <= 0 ||
                                         ((uintptr_t)partial & 15))))
@@ -784,21 +828,35 @@ CBIS_EXPORT int cbis_paged_prefill_tc5(const void* q, int q_ld, int total_rows, 
   if (st != CBIS_OK) return st;
   st = tc5::make_map(&map_v, vc, cache_rows, hd, hd, ps < tc5::BN ? ps : tc5::BN);
   if (st != CBIS_OK) return st;
-  const size_t smem = tc5::smem_bytes(hd) + (rates ? tc5::TABLE * sizeof(float) : 0);
+  const bool coded = k_scales != nullptr;
+  if (coded && (!v_scales || rates)) return CBIS_ERR_BAD_SIZE;      // (scales and such a bias both want the table)
+  const size_t smem = tc5::smem_bytes(hd) + (rates || coded ? tc5::TABLE * sizeof(float) : 0);
   const bool ext = cap > 0.f || (keep > 0 && window != 0);
   if (ext && rates) return CBIS_ERR_BAD_SIZE;      // the two come in kernels of their own
-  auto kern = hd == 128 ? (rates ? tc5::paged_prefill_tc5_kernel<128, true, false>
-                                 : (ext ? tc5::paged_prefill_tc5_kernel<128, false, true> : tc5::paged_prefill_tc5_kernel<128, false, false>))
-                        : (rates ? tc5::paged_prefill_tc5_kernel<64, true, false>
-                                 : (ext ? tc5::paged_prefill_tc5_kernel<64, false, true> : tc5::paged_prefill_tc5_kernel<64, false, false>));
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+#define CBIS_TC5(HD)                                                                                                        \
+  (rates ? tc5::paged_prefill_tc5_kernel<HD, true, false, false>                                                            \
+         : (coded ? (ext ? tc5::paged_prefill_tc5_kernel<HD, false, true, true> : tc5::paged_prefill_tc5_kernel<HD, false, false, true>) \
+                  : (ext ? tc5::paged_prefill_tc5_kernel<HD, false, true, false> : tc5::paged_prefill_tc5_kernel<HD, false, false, false>)))
+  auto kern = hd == 128 ? CBIS_TC5(128) : CBIS_TC5(64);
+#undef CBIS_TC5
+  // a kernel's limits are set once a device (a call takes the host some 10 us); what it needs of shared memory depends on nothing else
+  static std::atomic<unsigned long long> limits_set[2][5];
+  std::atomic<unsigned long long>& set = limits_set[hd == 128][rates ? 4 : (coded ? 2 : 0) + (ext ? 1 : 0)];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared);
-  if (e != cudaSuccess) return (int)e;
+  const bool known = dev >= 0 && dev < 64;
+  if (!known || !(set.load(std::memory_order_acquire) >> dev & 1)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return (int)e;
+    if (known) set.fetch_or(1ull << dev, std::memory_order_release);
+  }
   dim3 grid(2u * (unsigned)((max_seg_rows + tc5::BM - 1) / tc5::BM) * n_head * n_seg * n_chunks);
   e = launch_pdl(kern, grid, dim3(tc5::THREADS), smem, (cudaStream_t)stream, map_q, map_k, map_v, block_table, max_blocks,
                  cu_rows, seg_start, (__nv_bfloat16*)out, out_ld, seg0, n_seg, n_head, n_kv_head, ps,
-                 scale * 1.4426950408889634f, window, n_chunks, chunk_keys, partial, row0, error, sinks, slopes, rates, v_heads, cap, keep);
+                 scale * 1.4426950408889634f, window, n_chunks, chunk_keys, partial, row0, error, sinks, slopes, rates, v_heads, cap, keep, k_scales, v_scales);
   if (e == cudaSuccess && n_chunks > 1)
     e = launch_pdl(prefill_merge_kernel<__nv_bfloat16, true>, dim3(n_rows), dim3(128), 0, (cudaStream_t)stream,
                    (const float*)partial, positions, (const int*)nullptr, (__nv_bfloat16*)out, out_ld, row0, n_head, hd, window,
@@ -811,7 +869,7 @@ CBIS_EXPORT int cbis_paged_prefill_tc5(const void* q, int q_ld, int total_rows, 
 // memory) and what the device's SMs have; negative: a CUDA error.  (The occupancy calls of the runtime answer for
 // whole clusters and count an SM pair once; the profiler's counters show two blocks per SM at work.)
 CBIS_EXPORT int cbis_paged_prefill_tc5_blocks_per_sm() {
-  auto kern = tc5::paged_prefill_tc5_kernel<128, false, false>;
+  auto kern = tc5::paged_prefill_tc5_kernel<128, false, false, false>;
   cudaFuncAttributes fa;
   cudaError_t e = cudaFuncGetAttributes(&fa, kern);
   if (e != cudaSuccess) return -(int)e;

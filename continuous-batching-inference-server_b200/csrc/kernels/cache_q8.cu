@@ -113,7 +113,7 @@ template <typename TT, int N>
 __global__ void __launch_bounds__(256)
 kv_read_q8_kernel(const int8_t* kc, const float* ks, const int8_t* vc, const float* vs, TT* ko, TT* vo, const int* block_table, int max_blocks,
                   int num_pages, const int* seg_start, const int* seg_ctx, int heads, int hd, int hd_v, int ps, int window, int keep,
-                  int kept_blocks, int whole, int lpr_shift) {
+                  int kept_blocks, int whole, int as_codes, int lpr_shift) {
   pdl_wait();      // no early start for the kernel behind: those that read pages ask for the first of them before they wait
   const int s = blockIdx.y, ctx = min(seg_ctx[s], max_blocks * ps);
   if (ctx <= 0) return;
@@ -147,7 +147,7 @@ kv_read_q8_kernel(const int8_t* kc, const float* ks, const int8_t* vc, const flo
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int u = min(u0 + k * 256, units - 1);
-          scale[k] = scales[u >> lpr_shift];
+          scale[k] = as_codes ? 1.f : scales[u >> lpr_shift];
           if constexpr (N == 8) raw[k] = reinterpret_cast<const uint2*>(src)[u];
           else raw[k].x = reinterpret_cast<const unsigned*>(src)[u];
         }
@@ -181,7 +181,7 @@ kv_read_q8_kernel(const int8_t* kc, const float* ks, const int8_t* vc, const flo
         for (int k = 0; k < 4; ++k) {
           if (at[k] < 0) continue;
           const int8_t* p = src + (size_t)at[k] * width + c;
-          scale[k] = scales[at[k]];
+          scale[k] = as_codes ? 1.f : scales[at[k]];
           if constexpr (N == 8) raw[k] = *reinterpret_cast<const uint2*>(p);
           else if constexpr (N == 4) raw[k].x = *reinterpret_cast<const unsigned*>(p);
           else raw[k].x = (unsigned)(int)*p;
@@ -271,10 +271,10 @@ CBIS_EXPORT int cbis_kv_write_q8(const void* call) {
 // Values of the first n_seg requests' tokens go to the pages of the same numbers in ko and vo (vc and vo null: one array).  Of request s
 // the tokens that its queries at seg_start[s] .. seg_ctx[s] - 1 see: those from first_seen(seg_start[s]) on, at most max_tokens of
 // them, and the kept first ones.  whole: the rest of these tokens' pages too, up to seg_ctx[s] (a kernel that brings pages in whole
-// multiplies what it masks by zero, which only numbers survive).
+// multiplies what it masks by zero, which only numbers survive).  as_codes: the codes as they are, without their scales.
 struct KvReadCall {
   long long kc, ks, vc, vs, ko, vo, block_table, max_blocks, num_pages, seg_start, seg_ctx, n_seg, max_tokens, heads, hd, hd_v, ps, window, keep,
-      whole_dtype, stream;      // whole | dtype << 1
+      flags, stream;      // whole | dtype << 1 | as_codes << 2
 };
 CBIS_EXPORT int cbis_kv_read_q8(const void* call) {
   KvReadCall x;
@@ -284,7 +284,7 @@ CBIS_EXPORT int cbis_kv_read_q8(const void* call) {
   const int *block_table = (const int*)x.block_table, *seg_start = (const int*)x.seg_start, *seg_ctx = (const int*)x.seg_ctx;
   int hd_v = (int)x.hd_v;
   const int max_blocks = (int)x.max_blocks, num_pages = (int)x.num_pages, n_seg = (int)x.n_seg, max_tokens = (int)x.max_tokens, heads = (int)x.heads,
-            hd = (int)x.hd, ps = (int)x.ps, window = (int)x.window, keep = (int)x.keep, whole = (int)x.whole_dtype & 1, dtype = (int)(x.whole_dtype >> 1);
+            hd = (int)x.hd, ps = (int)x.ps, window = (int)x.window, keep = (int)x.keep, whole = (int)x.flags & 1, dtype = (int)x.flags >> 1 & 1, as_codes = (int)x.flags >> 2;
   if (n_seg <= 0 || max_tokens <= 0) return CBIS_OK;
   if (hd_v <= 0) hd_v = hd;
   if (heads <= 0 || hd <= 0 || ps <= 0 || max_blocks <= 0 || keep < 0 || n_seg > 65535) return CBIS_ERR_BAD_SIZE;
@@ -315,7 +315,7 @@ CBIS_EXPORT int cbis_kv_read_q8(const void* call) {
 #define CBIS_READ(TT, NN)                                                                                                              \
   return (int)launch_pdl(kv_read_q8_kernel<TT, NN>, grid, dim3(256), 0, st, (const int8_t*)kc, (const float*)ks, (const int8_t*)vc,    \
                          (const float*)vs, (TT*)ko, (TT*)vo, block_table, max_blocks, num_pages, seg_start, seg_ctx, heads, hd, hd_v, \
-                         ps, window, keep, kb, whole, shift)
+                         ps, window, keep, kb, whole, as_codes, shift)
   if (dtype == CBIS_F32) {
     if (vec) CBIS_READ(float, 4);
     CBIS_READ(float, 1);

@@ -702,18 +702,19 @@ def kv_read_q8(k_pages, v_pages, k_out, v_out, block_table, seg_start, seg_ctx, 
     if S == 0 or max_tokens <= 0 or shape[0] == 0:
         return
     _kv_read_q8(kc, ks, vc, vs, k_out, v_out, block_table.data_ptr(), block_table.shape[1], seg_start.data_ptr(), seg_ctx.data_ptr(), S,
-                int(max_tokens), int(window), int(keep), bool(whole_pages), code)
+                int(max_tokens), int(window), int(keep), int(bool(whole_pages)) | code << 1)
 
 
-def _kv_read_q8(kc, ks, vc, vs, k_out, v_out, table: int, blocks: int, start: int, ctx: int, n: int, max_tokens, window, keep, whole, code):
+def _kv_read_q8(kc, ks, vc, vs, k_out, v_out, table: int, blocks: int, start: int, ctx: int, n: int, max_tokens, window, keep, flags):
     P, G, ps, hd = kc.shape
     st = _q8_fn("cbis_kv_read_q8")(_READ_Q8.pack(
         kc.data_ptr(), ks.data_ptr(), _at(vc), _at(vs), k_out.data_ptr(), _at(v_out), table, blocks, P, start, ctx, n, max_tokens, G, hd,
-        hd if vc is None else vc.shape[3], ps, window, keep, int(whole) | code << 1, _stream_int()))
+        hd if vc is None else vc.shape[3], ps, window, keep, flags, _stream_int()))
     _check(st, "kv_read_q8", f"requests={n} heads={G} width={hd} page={ps}")
 
 
 ATTENTION_Q8_MAX_HEAD_DIM = 256
+PREFILL_Q8_FEW_ROWS = 64            # rows times query heads per key/value head up to which the kernel that reads codes takes a chunk
 ATTENTION_Q8_MAX_ROWS = 4096        # decoding rows, or row tiles of chunks, of one launch
 
 
@@ -842,12 +843,13 @@ def paged_decode_q8(qkv, k_off, v_off, k_pages, v_pages, block_table, row_seq, p
 
 def prefill_q8_reads_back(max_seg_rows: int, n_head: int, n_kv_head: int, head_dim: int, page_size: int, dtype, slopes=None, sinks=None,
                           q_temp=None, rates=None, cap: float = 0.0, keep: int = 0) -> bool:
-    """Whether ``paged_prefill_q8`` reads the cache back first: chunks of many rows, for which a kernel over values is there."""
-    if max_seg_rows * (n_head // n_kv_head) <= 64 or page_size & (page_size - 1) or head_dim > 128:
+    """Whether ``paged_prefill_q8`` reads the cache back first: chunks of many rows, for which a faster kernel over pages of q's type is
+    there: in bfloat16 the tcgen05 one, over codes as they are; in 32 bits the tiled one."""
+    if max_seg_rows * (n_head // n_kv_head) <= PREFILL_Q8_FEW_ROWS or page_size & (page_size - 1) or slopes is not None or q_temp is not None:
         return False
     if dtype == torch.float32:
-        return slopes is None and sinks is None and q_temp is None and not cap and not keep
-    return True
+        return head_dim <= 128 and sinks is None and not cap and not keep
+    return head_dim in (64, 128) and 8 <= page_size <= 128 and USE_TCGEN05
 
 
 def prefill_q8_takes(n_seg: int, max_seg_rows: int, n_head: int, n_kv_head: int, head_dim: int, page_size: int, dtype, **extra) -> bool:
@@ -894,29 +896,20 @@ def paged_prefill_q8(q, k_pages, v_pages, block_table, cu_rows, seg_start, seg_c
     if n_seg == 0 or n_rows == 0 or max_seg_rows <= 0:
         return
     window, cap, keep = int(window), float(cap), int(keep)
-    if work is None or not prefill_q8_reads_back(max_seg_rows, n_head, n_kv_head, head_dim, page_size, q.dtype, slopes, sinks, q_temp, rates, cap, keep):
+    if work is None or out.data_ptr() % 16 or out.stride(0) % 8 or not prefill_q8_reads_back(max_seg_rows, n_head, n_kv_head, head_dim, page_size, q.dtype, slopes, sinks, q_temp, rates, cap, keep):
         return _attention_q8(what, q, -1, -1, k_pages, v_pages, block_table, None, None, None, cu_rows, seg_start, seg0, n_seg,
                              int(max_seg_rows), out, scratch, counters, n_head, n_kv_head, head_dim, page_size, scale, window,
                              int(max_context), slopes, sinks, q_temp, rates, cap, keep)
     k, v = work
     tokens = min(max_context, abs(window) + max_seg_rows) if window else max_context
-    blocks = block_table.shape[1]
+    blocks, wide = block_table.shape[1], q.dtype is _FLOAT32
     _kv_read_q8(kc, ks, vc, vs, k, v, block_table.data_ptr() + 4 * seg0 * blocks, blocks, seg_start.data_ptr() + 4 * seg0,
-                seg_ctx.data_ptr() + 4 * seg0, n_seg, tokens, window, keep, True, F32 if q.dtype is _FLOAT32 else BF16)
+                seg_ctx.data_ptr() + 4 * seg0, n_seg, tokens, window, keep, 1 | (F32 if wide else BF16) << 1 | (not wide) << 2)
     chunks = _prefill_q8_chunks(max_seg_rows, n_seg, n_head, head_dim, max_context, q.dtype)
     args = (q, k, v, block_table, cu_rows, seg_start, out, seg0, n_seg, max_seg_rows, n_head, n_kv_head, head_dim, page_size, scale, window)
-    tail = (scratch, positions, row0, n_rows)
-    if q.dtype == torch.float32:
-        return paged_prefill_f32(*args, chunks, *tail)
-    tc5 = (head_dim in (64, 128) and 8 <= page_size <= 128 and USE_TCGEN05 and q_temp is None and (slopes is None) == (rates is None)
-           and not (rates is not None and (cap or keep)) and out.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0)
-    if tc5:
-        return paged_prefill_tc5(*args, chunks, *tail, sinks=sinks, slopes=slopes, rates=rates, cap=cap, keep=keep)
-    if head_dim in (64, 128):      # the other kernel's tiles have 64 rows: fewer chunks than it would take are fine
-        chunks = (1, 0)
-    extra = {} if slopes is None and sinks is None and q_temp is None and not cap and not keep else dict(
-        v_head_dim=head_dim, slopes=slopes, sinks=sinks, q_temp=q_temp, rates=rates, cap=cap, keep=keep)
-    return paged_prefill_bf16(*args, chunks, *tail, **extra)
+    if wide:
+        return paged_prefill_f32(*args, chunks, scratch, positions, row0, n_rows)
+    _prefill_tc5(*args, *chunks, scratch, positions, row0, n_rows, sinks, None, None, 1, cap, keep, ks, vs)
 
 
 def _need_columns(q, out, n_head, v_heads, head_dim, v_head_dim):
@@ -1242,14 +1235,23 @@ def paged_prefill_tc5(q, k_cache, v_cache, block_table, cu_rows, seg_start, out,
     if n_chunks > 1:
         assert partial.dtype == torch.float32 and partial.numel() >= n_rows * n_head * n_chunks * (head_dim + 4)
         assert positions.dtype == torch.int32 and positions.numel() >= row0 + n_rows
+    _prefill_tc5(q, k_cache, v_cache, block_table, cu_rows, seg_start, out, seg0, n_seg, max_seg_rows, n_head, n_kv_head, head_dim, page_size,
+                 scale, window, n_chunks, chunk_keys, partial, positions, row0, n_rows, sinks, slopes, rates, v_heads, cap, keep, None, None)
+
+
+def _prefill_tc5(q, k_cache, v_cache, block_table, cu_rows, seg_start, out, seg0, n_seg, max_seg_rows, n_head, n_kv_head, head_dim, page_size,
+                 scale, window, n_chunks, chunk_keys, partial, positions, row0, n_rows, sinks, slopes, rates, v_heads, cap, keep, k_scales,
+                 v_scales):
+    """The launch of ``paged_prefill_tc5``, and, with ``k_scales`` and ``v_scales``, over pages that hold the codes of an 8-bit cache as they are."""
     fn = kernels().cbis_paged_prefill_tc5
     if fn.argtypes is None:      # plain numbers are converted by their declared types: a third of the time that an object each takes
         P, I = c_void_p, c_int
-        fn.argtypes = [P, I, I, P, P, I, P, I, P, P, P, I, I, I, I, I, I, I, I, c_float, I, I, I, P, P, I, I, P, P, P, P, P, I, c_float, I]
+        fn.argtypes = [P, I, I, P, P, I, P, I, P, P, P, I, I, I, I, I, I, I, I, c_float, I, I, I, P, P, I, I, P, P, P, P, P, I, c_float, I, P, P]
     st = fn(q.data_ptr(), q.stride(0), q.shape[0], k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], block_table.data_ptr(),
             block_table.shape[1], cu_rows.data_ptr(), seg_start.data_ptr(), out.data_ptr(), out.stride(0), seg0, n_seg, max_seg_rows, n_head,
             n_kv_head, head_dim, page_size, scale, window, n_chunks, chunk_keys, _at(partial) or None, _at(positions) or None, row0, n_rows,
-            tcgen05_error_flag(q.device).data_ptr(), _stream(), _at(sinks) or None, _at(slopes) or None, _at(rates) or None, v_heads, cap, keep)
+            tcgen05_error_flag(q.device).data_ptr(), _stream(), _at(sinks) or None, _at(slopes) or None, _at(rates) or None, v_heads, cap, keep,
+            _at(k_scales) or None, _at(v_scales) or None)
     _check(st, "paged_prefill_tc5", f"segments={n_seg} heads={n_head}/{n_kv_head} page={page_size} chunks={n_chunks}x{chunk_keys}")
 
 

@@ -174,13 +174,6 @@ def prefill(ops, c, window=0, work=False, seg0=0, out=None, max_context=None, **
     return out
 
 
-def read_back(c):
-    """What attention over the values read back sees: bfloat16 values where the rows are."""
-    if c["dtype"] == BF:
-        c["held"] = [[x.to(BF).double() for x in part] for part in c["held"]]
-    return c
-
-
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("H,G,hd,ps,window", [
@@ -206,9 +199,31 @@ def test_chunk_extras(ops, dtype, kw):
 @pytest.mark.parametrize("H,G,hd,ps,window", [(2, 2, 64, 16, 0), (4, 2, 128, 32, 0), (2, 1, 32, 8, 0), (2, 2, 80, 16, 50), (2, 1, 128, 16, -64), (2, 2, 64, 64, 70)])
 def test_long_chunks_read_back(ops, dtype, H, G, hd, ps, window):
     """Chunks of many rows; the pages that the values are read back into hold NaN before."""
-    c = read_back(make(ops, dtype, H, G, hd, ps, [190, 300, 77], [130, 90, 77], seed=hd))
+    c = make(ops, dtype, H, G, hd, ps, [190, 300, 77], [130, 90, 77], seed=hd)
     rows = list(range(0, 297, 13)) + [129, 130, 219, 220, 296]
     check(c, prefill(ops, c, window, work=True), hd ** -0.5, window, rows=rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_key_that_is_not_finite_in_a_long_chunk(ops, hd):
+    """The same over pages read back: to every row that sees it, and to no other."""
+    for x in "kv":
+        c = make(ops, BF, 4, 2, hd, 16, [300, 260], [150, 140], seed=9)
+        c[x].scales[int(c["table"][0, 200 // 16]), 1, 200 % 16] = math.nan
+        out = prefill(ops, c, work=True).cpu().view(290, 4, hd)
+        for r in range(290):
+            hit = r < 150 and 150 + r >= 200
+            assert torch.isnan(out[r, 2:]).all().item() == hit and torch.isfinite(out[r, :2].float()).all(), r
+            assert hit or torch.isfinite(out[r].float()).all(), r
+
+
+@pytest.mark.gpu
+def test_a_long_context_in_chunks_of_keys(ops):
+    """Few rows behind a long context: the keys of the kernel over pages read back are cut, and the parts merged."""
+    c = make(ops, BF, 2, 1, 128, 16, [17000], [70], seed=3)
+    check(c, prefill(ops, c, work=True), 128 ** -0.5, rows=[0, 1, 33, 68, 69])
+    check(c, prefill(ops, c, 16500, work=True), 128 ** -0.5, 16500, rows=[0, 69])
 
 
 @pytest.mark.gpu
@@ -216,7 +231,7 @@ def test_long_chunks_read_back(ops, dtype, H, G, hd, ps, window):
 def test_long_chunk_extras(ops, kw):
     kw, told, window, keep = numbers(kw, 4)
     for hd in (64, 96):
-        c = read_back(make(ops, BF, 4, 2, hd, 16, [190, 300], [120, 90], seed=hd))
+        c = make(ops, BF, 4, 2, hd, 16, [190, 300], [120, 90], seed=hd)
         check(c, prefill(ops, c, window, work=True, **kw), hd ** -0.5, window, keep, rows=list(range(0, 210, 11)) + [119, 120, 209], **told)
 
 
@@ -225,7 +240,6 @@ def test_rows_of_other_requests_stay(ops):
     """A step holds decoding rows first: the chunks' call starts at a later request and row and leaves the others' results."""
     for work in (False, True):
         c = make(ops, BF, 4, 2, 64, 16, [90, 33, 200, 140], [1, 1, 70 if work else 9, 5], seed=3)
-        c = read_back(c) if work else c
         out = prefill(ops, c, work=work, seg0=2)
         assert torch.all(out[:2] == 7.5)
         check(c, out, 1 / 8, rows=list(range(2, len(c["positions"]), 3)))
@@ -364,11 +378,10 @@ def test_store_attend_and_read_back_together(ops):
         ops.paged_decode_q8(rows[p:p + 1], H * hd, (H + G) * hd, c["k"], c["v"], table, i32(0), i32(p), slots[p:p + 1], out[p:p + 1], *dec, H, G, hd, ps,
                             hd ** -0.5, 0, n)
     c.update(seq=torch.zeros(n, dtype=torch.int32), positions=pos)
-    check(c, out, hd ** -0.5, rows=list(range(23)) + list(range(173, n)))
-    check(read_back(c), out, hd ** -0.5, rows=range(23, 173, 7))
+    check(c, out, hd ** -0.5, rows=list(range(23)) + list(range(23, 173, 7)) + list(range(173, n)))
     ko, vo = (torch.zeros(14, G, ps, hd, device="cuda") for _ in "kv")
     ops.kv_read_q8(c["k"], c["v"], ko, vo, table, i32(0), i32(n), n)
-    assert torch.equal(ko[table[0].long()].transpose(1, 2).reshape(-1, G, hd)[:n].to(BF).double().cpu(), c["held"][0][0])
+    assert torch.equal(ko[table[0].long()].transpose(1, 2).reshape(-1, G, hd)[:n].double().cpu(), c["held"][0][0].float().double())
 
 
 def test_refusals():
