@@ -17,9 +17,7 @@ int padded_width(int hd) { return hd <= 32 ? 32 : (hd <= 64 ? 64 : (hd <= 128 ? 
 
 // Columns of queries / 8: as many as the query heads and rows that share keys fill, up to what the accumulators' registers allow.
 int columns8(int hdp, int f32, long long queries) {
-  const int most = hdp == 256 ? (f32 ? 1 : 2) : (f32 ? 2 : 4);
-  const int nt = queries <= 8 ? 1 : (queries <= 16 ? 2 : 4);
-  return nt < most ? nt : most;
+  return queries <= 8 || (hdp == 256 && f32) ? 1 : 2;
 }
 int blocks_per_sm(int hdp, int nt, int f32) { return nt == 1 && hdp < 256 ? (f32 || hdp == 128 ? 3 : 4) : 2; }      // as Q8Shape::BLOCKS
 

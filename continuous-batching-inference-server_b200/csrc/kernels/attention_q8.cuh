@@ -182,7 +182,7 @@ struct Q8Shape {
   static constexpr int LDQ = HDP >= 128 ? HDP + 16 : HDP;       // bytes of a query's row in shared memory: no two lanes of a load on one bank
   static constexpr int TILE = 32 * HDP + 128;                   // bytes of 16 keys: codes of keys, of values, their scales
   static constexpr int STAGE = TPW * TILE;
-  static constexpr int BLOCKS = NT == 1 && HDP < 256 ? (PARTS == 1 && HDP < 128 ? 4 : 3) : 2;      // per SM, as far as registers go
+  static constexpr int BLOCKS = NT == 1 && HDP < 256 ? (PARTS == 2 && HDP < 128 ? 4 : 3) : 2;      // per SM, as far as registers go
 };
 // Shared memory of a block (in this order): the warps' rings; sums of jq columns from four warps, maxima of 8; the queries' bytes; the
 // columns' powers of two, merged maxima and sums; a few integers; the items.
@@ -206,7 +206,7 @@ template <int HDP, int NT, int PARTS, bool EXT, bool FAST>
 __global__ void __launch_bounds__(Q8_THREADS, Q8Shape<HDP, NT, PARTS>::BLOCKS)
 attention_q8_kernel(const __grid_constant__ Q8Args a) {
   using Shape = Q8Shape<HDP, NT, PARTS>;
-  using TT = typename std::conditional<PARTS == 1, __nv_bfloat16, float>::type;
+  using TT = typename std::conditional<PARTS == 2, __nv_bfloat16, float>::type;
   constexpr int TPW = Shape::TPW, UNIT = Shape::UNIT, NQ = Shape::NQ, LDS = Shape::LDS, LDQ = Shape::LDQ, KS = HDP / 16;
   constexpr int STEPS = HDP / 32, VW = HDP / 32, PW = VW < 4 ? VW : 4;      // steps of the scores' product; words of a value that a lane takes, of one load
   constexpr bool Q_IN_REGS = NT * HDP <= 128;
@@ -659,13 +659,10 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
             l_run[nt][e & 1] += p[e];
             p[e] = whole || s[u][nt][e] != -INFINITY ? p[e] * vx[u][e >> 1] : 0.f;      // a hidden key's scale may be anything
           }
-          if constexpr (PARTS == 1) {
-            pf[0][nt][0] = transposed(pack_bf16(p[0], p[1]));
-            pf[0][nt][1] = transposed(pack_bf16(p[2], p[3]));
-          } else {
-            unsigned a0[3], a1[3];
-            cut3(p[0], p[1], a0);
-            cut3(p[2], p[3], a1);
+          {
+            unsigned a0[PARTS], a1[PARTS];
+            cut_parts(p[0], p[1], a0);
+            cut_parts(p[2], p[3], a1);
 #pragma unroll
             for (int i = 0; i < PARTS; ++i) {
               pf[i][nt][0] = transposed(a0[i]);
@@ -892,11 +889,7 @@ int q8_run(const Q8Args& a, const Q8Plan& p, bool ext, int f32, cudaStream_t st)
       if (p.nt == 2) return q8_launch2<HDP, 2, 3>(a, p, ext, st);
     return CBIS_ERR_BAD_SIZE;
   }
-  if (p.nt == 1) return q8_launch2<HDP, 1, 1>(a, p, ext, st);
-  if (p.nt == 2) return q8_launch2<HDP, 2, 1>(a, p, ext, st);
-  if constexpr (HDP < 256)
-    if (p.nt == 4) return q8_launch2<HDP, 4, 1>(a, p, ext, st);
-  return CBIS_ERR_BAD_SIZE;
+  return p.nt == 1 ? q8_launch2<HDP, 1, 2>(a, p, ext, st) : q8_launch2<HDP, 2, 2>(a, p, ext, st);
 }
 
 }  // namespace cbis

@@ -24,13 +24,16 @@ __device__ __forceinline__ unsigned pack_bf16(float a, float b) {
   return *reinterpret_cast<const unsigned*>(&p);
 }
 // Two values' parts, packed; what is left of the values after a part goes on to the next.
-__device__ __forceinline__ void cut3(float a, float b, unsigned (&part)[3]) {
+template <int N>
+__device__ __forceinline__ void cut_parts(float a, float b, unsigned (&part)[N]) {
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < N; ++i) {
     part[i] = pack_bf16(a, b);
+    if (i + 1 == N) break;
     a -= __uint_as_float(part[i] << 16);
     b -= __uint_as_float(part[i] & 0xffff0000u);
   }
 }
+__device__ __forceinline__ void cut3(float a, float b, unsigned (&part)[3]) { cut_parts(a, b, part); }
 
 }  // namespace cbis

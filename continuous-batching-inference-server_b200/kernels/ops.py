@@ -714,7 +714,6 @@ def _kv_read_q8(kc, ks, vc, vs, k_out, v_out, table: int, blocks: int, start: in
 
 
 ATTENTION_Q8_MAX_HEAD_DIM = 256
-PREFILL_Q8_FEW_ROWS = 64            # rows times query heads per key/value head up to which the kernel that reads codes takes a chunk
 ATTENTION_Q8_MAX_ROWS = 4096        # decoding rows, or row tiles of chunks, of one launch
 
 
@@ -841,20 +840,30 @@ def paged_decode_q8(qkv, k_off, v_off, k_pages, v_pages, block_table, row_seq, p
                   sinks, q_temp, rates, float(cap), int(keep))
 
 
-def prefill_q8_reads_back(max_seg_rows: int, n_head: int, n_kv_head: int, head_dim: int, page_size: int, dtype, slopes=None, sinks=None,
-                          q_temp=None, rates=None, cap: float = 0.0, keep: int = 0) -> bool:
-    """Whether ``paged_prefill_q8`` reads the cache back first: chunks of many rows, for which a faster kernel over pages of q's type is
-    there: in bfloat16 the tcgen05 one, over codes as they are; in 32 bits the tiled one."""
-    if max_seg_rows * (n_head // n_kv_head) <= PREFILL_Q8_FEW_ROWS or page_size & (page_size - 1) or slopes is not None or q_temp is not None:
+def prefill_q8_reads_back(n_rows: int, max_seg_rows: int, n_seg: int, keys: int, n_head: int, n_kv_head: int, head_dim: int, page_size: int, dtype,
+                          slopes=None, sinks=None, q_temp=None, rates=None, cap: float = 0.0, keep: int = 0) -> bool:
+    """Whether ``paged_prefill_q8`` reads the cache back first (no row sees more than ``keys`` keys): where the kernel over pages of q's type
+    is faster, or the one that reads codes cannot count the row tiles.
+
+    In bfloat16 that is the tcgen05 kernel over codes as they are.  Against the kernel that reads codes it saves some 3.5 us a million
+    pairs of row and key (times heads, of 128), and costs some 8 us more, and 1 us a million numbers read back.  16 heads of 128 behind 2,000 keys:
+    32 rows 24.2 us here and 34.2 there, 64 rows 32.0 and 34.2, 128 rows 39.9 and 34.4, 512 rows behind 8,192 268 and 148; twelve requests
+    of 16 rows behind 1,000 keys 43.9 and 69.1, over 4 key/value heads 43.9 and 47.2.  In 32 bits the kernel that reads codes multiplies
+    on the tensor cores and is the faster one: 512 rows of 8 heads of 32 behind 8,192 85 us and 131, 256 rows of 16 heads over 4 of 64 behind 2,000
+    43 and 75."""
+    wide = dtype == torch.float32
+    if page_size & (page_size - 1) or slopes is not None or q_temp is not None or (
+            head_dim > 128 or sinks is not None or cap or keep if wide else head_dim not in (64, 128) or not 8 <= page_size <= 128 or not USE_TCGEN05):
         return False
-    if dtype == torch.float32:
-        return head_dim <= 128 and sinks is None and not cap and not keep
-    return head_dim in (64, 128) and 8 <= page_size <= 128 and USE_TCGEN05
+    group = n_head // n_kv_head
+    if n_seg * -(-max_seg_rows // max(1, 16 // group)) > ATTENTION_Q8_MAX_ROWS:
+        return True
+    return not wide and 3.5e-6 / 128 * n_rows * n_head * keys * head_dim > 8 + 1e-6 * n_seg * keys * n_kv_head * head_dim
 
 
-def prefill_q8_takes(n_seg: int, max_seg_rows: int, n_head: int, n_kv_head: int, head_dim: int, page_size: int, dtype, **extra) -> bool:
+def prefill_q8_takes(n_rows: int, max_seg_rows: int, n_seg: int, keys: int, n_head: int, n_kv_head: int, head_dim: int, page_size: int, dtype, **extra) -> bool:
     """Whether ``paged_prefill_q8`` with ``work`` takes these sizes (the kernel that reads codes counts its row tiles)."""
-    return (prefill_q8_reads_back(max_seg_rows, n_head, n_kv_head, head_dim, page_size, dtype, **extra)
+    return (prefill_q8_reads_back(n_rows, max_seg_rows, n_seg, keys, n_head, n_kv_head, head_dim, page_size, dtype, **extra)
             or _q8_scratch(n_seg, max_seg_rows, n_head, n_kv_head, head_dim, dtype_code(dtype), 1)[0] == 0)
 
 
@@ -865,7 +874,8 @@ def paged_prefill_q8(q, k_pages, v_pages, block_table, cu_rows, seg_start, seg_c
     seg0 + n_seg - 1, whose rows (``row0`` .. ``row0 + n_rows - 1`` in all, at most ``max_seg_rows`` each) are ``cu_rows[s]`` .. ``cu_rows[s + 1] - 1`` at positions
     from ``seg_start[s]`` to ``seg_ctx[s] - 1``; no context is longer than ``max_context``.  A few rows go through the kernel that reads codes;
     for many (``prefill_q8_reads_back``) the cache is read back into ``work``, a pair of pages of q's type and the codes' shape, and
-    attended to there.  Without ``work`` the first takes all.  The rest as in ``paged_decode_q8``."""
+    attended to there (every page that a row sees is then one of the cache's).  Without ``work`` the first takes all.  The rest as in
+    ``paged_decode_q8``."""
     what = "paged_prefill_q8"
     dtype_code(q.dtype)
     kc, ks = k_pages
@@ -896,12 +906,13 @@ def paged_prefill_q8(q, k_pages, v_pages, block_table, cu_rows, seg_start, seg_c
     if n_seg == 0 or n_rows == 0 or max_seg_rows <= 0:
         return
     window, cap, keep = int(window), float(cap), int(keep)
-    if work is None or out.data_ptr() % 16 or out.stride(0) % 8 or not prefill_q8_reads_back(max_seg_rows, n_head, n_kv_head, head_dim, page_size, q.dtype, slopes, sinks, q_temp, rates, cap, keep):
+    tokens = min(max_context, abs(window) + max_seg_rows) if window else max_context
+    if work is None or out.data_ptr() % 16 or out.stride(0) % 8 or not prefill_q8_reads_back(
+            n_rows, max_seg_rows, n_seg, tokens, n_head, n_kv_head, head_dim, page_size, q.dtype, slopes, sinks, q_temp, rates, cap, keep):
         return _attention_q8(what, q, -1, -1, k_pages, v_pages, block_table, None, None, None, cu_rows, seg_start, seg0, n_seg,
                              int(max_seg_rows), out, scratch, counters, n_head, n_kv_head, head_dim, page_size, scale, window,
                              int(max_context), slopes, sinks, q_temp, rates, cap, keep)
     k, v = work
-    tokens = min(max_context, abs(window) + max_seg_rows) if window else max_context
     blocks, wide = block_table.shape[1], q.dtype is _FLOAT32
     _kv_read_q8(kc, ks, vc, vs, k, v, block_table.data_ptr() + 4 * seg0 * blocks, blocks, seg_start.data_ptr() + 4 * seg0,
                 seg_ctx.data_ptr() + 4 * seg0, n_seg, tokens, window, keep, 1 | (F32 if wide else BF16) << 1 | (not wide) << 2)

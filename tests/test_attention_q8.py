@@ -166,12 +166,26 @@ def prefill(ops, c, window=0, work=False, seg0=0, out=None, max_context=None, **
     out = torch.full(c["q"].shape, 7.5, dtype=c["dtype"], device="cuda") if out is None else out
     buf = scratch(ops, rows, max(c["rows"]), n, c, max_context)
     pages = tuple(torch.full(c["k"].codes.shape, math.nan, dtype=c["dtype"], device="cuda") for _ in "kv") if work else None
+    takes = ops.prefill_q8_reads_back
+    if work:        # wherever there is a kernel over pages read back, whichever is the faster one
+        ops.prefill_q8_reads_back = lambda rows, most, n_seg, keys, *rest: takes(10 ** 9, most, n_seg, keys, *rest) or takes(rows, 10 ** 9, n_seg, keys, *rest)
     start = torch.tensor([a - b for a, b in zip(c["ctx"], c["rows"])], dtype=torch.int32).cuda()
     ops.paged_prefill_q8(c["q"].cuda(), c["k"], c["v"], c["table"].cuda(), c["cu"].cuda(), start, torch.tensor(c["ctx"], dtype=torch.int32).cuda(),
                          c["positions"].cuda(), out, seg0, n, row0, rows, max(c["rows"]), c["H"], c["G"], c["hd"], c["ps"], c["hd"] ** -0.5, window,
                          max_context or max(c["ctx"]), *buf, pages, **kw)
+    ops.prefill_q8_reads_back = takes
     assert int(buf[1].abs().sum()) == 0
     return out
+
+
+def test_which_kernel_takes_a_chunk():
+    from cbis_b200.kernels import ops
+    small = dict(n_seg=1, keys=2000, n_head=16, n_kv_head=16, head_dim=128, page_size=16, dtype=BF)
+    reads = lambda rows, **kw: ops.prefill_q8_reads_back(rows, rows, **{**small, **kw})      # noqa: E731
+    assert not reads(32) and reads(256) and not reads(256, head_dim=96) and not reads(256, page_size=24) and not reads(256, q_temp=(0.1, 5))
+    assert not reads(256, slopes=1, rates=1) and reads(256, sinks=1) and reads(256, cap=3.0, keep=2)
+    assert not reads(4096, dtype=F32) and reads(70000, dtype=F32) and not reads(70000, dtype=F32, sinks=1)      # (more row tiles than are counted)
+    assert not ops.prefill_q8_takes(70000, 70000, **{**small, "dtype": F32}, sinks=1)
 
 
 @pytest.mark.gpu
