@@ -39,7 +39,7 @@
 // CODED: keys and values are whole numbers (the codes of an 8-bit cache, exact in bfloat16) with a scale per key and one per value:
 // the scores are multiplied by the one and the weights, on their way to bfloat16, by the other, so nothing is rounded more often than
 // over keys and values in bfloat16.  The softmax threads bring a tile's 128 scales through the table's place in shared memory,
-// asked for a tile ahead.  A value whose scale is not finite makes its key's scores not-a-number (its rows' results then are, and a row
+// asked for a tile ahead.  A value whose scale is not finite, or whose page the cache does not have, makes its key's scores not-a-number (its rows' results then are, and a row
 // that does not see it multiplies by zero).
 //
 // Every wait on an mbarrier is bounded; when a limit runs out the block sets *error, stops, frees its
@@ -218,7 +218,7 @@ paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                          int n_head, int n_kv_head, int ps, float scale_log2e, int window, int n_chunks, int chunk_keys,
                          float* partial, int row0, int* error, const float* __restrict__ sinks,
                          const float* __restrict__ slopes, const float* __restrict__ rates, int v_heads, float cap, int keep,
-                         const float* k_scales, const float* v_scales) {
+                         const float* k_scales, const float* v_scales, int num_pages) {
   constexpr int PBUF = p_buffers(HD), HALVES = HD / 64, Q_BYTES = HALVES * Q_HALF_BYTES, KV_BYTES = HALVES * KV_HALF_BYTES;
   extern __shared__ __align__(1024) unsigned char base[];   // no byte to spare for rounding the address up: checked below
   unsigned char* sQ = base;                                   // 2 halves of the head dim
@@ -383,7 +383,7 @@ paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     auto page_of = [&](int j) -> int {
       const int j0 = tile_at(j) * BN + lane * piece;
       return (j < n_tiles && lane < pieces_per_tile && ((j0 < kend && j0 + piece > kbegin) || (EXT && j0 < kept_upto)))
-                 ? __ldg(bt + j0 / ps) : 0;
+                 ? __ldg(bt + (CODED ? max(min(j0 / ps, max_blocks - 1), 0) : j0 / ps)) : 0;
     };
     const int kv = warp == 0 ? 0 : 1;
     int page_now = page_of(0);
@@ -453,10 +453,11 @@ paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     float k_scale = 0.f, v_scale = 0.f;
     auto find_scales = [&](int j) {
       if (r < BN && j < n_tiles) {
-        const int at = max(min(tile_at(j) * BN + r, (EXT ? max(kend, kept_upto) : kend) - 1), 0);
-        const size_t row = (size_t)max(bt[at / ps], 0) * n_kv_head * ps + at % ps;
+        const int at = max(min(tile_at(j) * BN + r, (EXT ? max(kend, kept_upto) : kend) - 1), 0), page = bt[min(at / ps, max_blocks - 1)];
+        const bool there = page >= 0 && page < num_pages;
+        const size_t row = (size_t)(there ? page : 0) * n_kv_head * ps + at % ps;
         k_scale = k_scales[row + hp.key * ps];
-        v_scale = v_scales[row + hp.value * ps];
+        v_scale = there ? v_scales[row + hp.value * ps] : INFINITY;
       }
     };
     if constexpr (CODED) find_scales(0);
@@ -576,6 +577,11 @@ paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       unsigned pk[8][4];
 #pragma unroll
       for (int q8 = 0; q8 < 8; ++q8) {
+        float4 vx[2];
+        if constexpr (CODED) {
+          vx[0] = *reinterpret_cast<const float4*>(table + BN + q8 * 8);
+          vx[1] = *reinterpret_cast<const float4*>(table + BN + q8 * 8 + 4);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const unsigned long long x = pack2(v[q8 * 8 + 2 * i], v[q8 * 8 + 2 * i + 1]);
@@ -585,8 +591,8 @@ paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           e1 = ex2(e1);
           psum = add2(psum, pack2(e0, e1));
           if constexpr (CODED) {
-            const float2 x2 = *reinterpret_cast<const float2*>(table + BN + q8 * 8 + 2 * i);
-            unpack2(mul2(pack2(e0, e1), pack2(x2.x, x2.y)), e0, e1);
+            const float4 f = vx[i >> 1];
+            unpack2(mul2(pack2(e0, e1), i & 1 ? pack2(f.z, f.w) : pack2(f.x, f.y)), e0, e1);
           }
           __nv_bfloat162 b2 = __floats2bfloat162_rn(e0, e1);
           pk[q8][i] = *reinterpret_cast<unsigned*>(&b2);
@@ -856,7 +862,7 @@ CBIS_EXPORT int cbis_paged_prefill_tc5(const void* q, int q_ld, int total_rows, 
   dim3 grid(2u * (unsigned)((max_seg_rows + tc5::BM - 1) / tc5::BM) * n_head * n_seg * n_chunks);
   e = launch_pdl(kern, grid, dim3(tc5::THREADS), smem, (cudaStream_t)stream, map_q, map_k, map_v, block_table, max_blocks,
                  cu_rows, seg_start, (__nv_bfloat16*)out, out_ld, seg0, n_seg, n_head, n_kv_head, ps,
-                 scale * 1.4426950408889634f, window, n_chunks, chunk_keys, partial, row0, error, sinks, slopes, rates, v_heads, cap, keep, k_scales, v_scales);
+                 scale * 1.4426950408889634f, window, n_chunks, chunk_keys, partial, row0, error, sinks, slopes, rates, v_heads, cap, keep, k_scales, v_scales, num_pages);
   if (e == cudaSuccess && n_chunks > 1)
     e = launch_pdl(prefill_merge_kernel<__nv_bfloat16, true>, dim3(n_rows), dim3(128), 0, (cudaStream_t)stream,
                    (const float*)partial, positions, (const int*)nullptr, (__nv_bfloat16*)out, out_ld, row0, n_head, hd, window,

@@ -51,7 +51,7 @@ Q8Plan q8_plan(int n, int rows_of_seg, int n_head, int n_kv_head, int hd, int f3
       break;
     }
   }
-  const long long pairs = p.items * n_kv_head * p.head_blocks, most = pairs * (max_context / (128 * tpw) + 2);      // no more blocks than there can be pieces
+  const long long pairs = p.items * n_kv_head * p.head_blocks, most = pairs * (max_context / (64 * tpw) + 2);      // no more blocks than there can be pieces
   if (most < p.blocks) p.blocks = most;
   p.floats = p.blocks * 2 * 8 * p.nt * (p.hdp + 4);
   p.counters = pairs;
@@ -86,15 +86,17 @@ struct Q8Call {
 CBIS_EXPORT int cbis_attention_q8(const void* call) {
   Q8Call x;
   memcpy(&x, call, sizeof x);
-  const int n = (int)x.n, rows_of_seg = (int)x.rows_of_seg, dtype = (int)x.dtype, hd = (int)x.hd, ps = (int)x.ps, n_head = (int)x.n_head,
-            n_kv_head = (int)x.n_kv_head, max_blocks = (int)x.max_blocks, num_pages = (int)x.num_pages, n_seqs = (int)x.n_seqs,
-            max_context = (int)x.max_context, keep = (int)x.keep, window = (int)x.window, n_rows = (int)x.n_rows, seg0 = (int)x.seg0, ld = (int)x.ld;
+  const int n = q8_int(x.n), rows_of_seg = q8_int(x.rows_of_seg), dtype = (int)x.dtype, hd = q8_int(x.hd), ps = q8_int(x.ps), n_head = q8_int(x.n_head),
+            n_kv_head = q8_int(x.n_kv_head), max_blocks = q8_int(x.max_blocks), num_pages = q8_int(x.num_pages), n_seqs = q8_int(x.n_seqs),
+            max_context = q8_int(x.max_context), keep = q8_int(x.keep), window = q8_int(x.window), n_rows = q8_int(x.n_rows), seg0 = q8_int(x.seg0),
+            ld = (int)x.ld;
   float* part = (float*)x.part;
   if (n <= 0) return CBIS_OK;
   if (dtype != CBIS_F32 && dtype != CBIS_BF16) return CBIS_ERR_BAD_DTYPE;
   if (hd <= 0 || hd > 256 || hd % 16 || ps <= 0 || n_kv_head <= 0 || n_head <= 0 || n_head % n_kv_head || max_blocks <= 0 || keep < 0 ||
       num_pages <= 0 || rows_of_seg < 0 || rows_of_seg > Q8_MAX_POSITION || max_context < 0 || n_rows < 0 || (rows_of_seg && (seg0 < 0 || seg0 + n > n_seqs)) || (!rows_of_seg && n > n_rows))
     return CBIS_ERR_BAD_SIZE;
+  if (x.ld > 0x7fffffffLL || x.out_ld > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
   if ((long long)max_blocks * ps >= Q8_MAX_POSITION || (long long)num_pages * ps * n_kv_head > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
   if (window < -Q8_MAX_POSITION) return CBIS_ERR_BAD_SIZE;
   const int f32 = dtype == CBIS_F32, align = f32 ? 4 : 8;
@@ -109,13 +111,13 @@ CBIS_EXPORT int cbis_attention_q8(const void* call) {
   a.slot_mapping = (const int*)x.slot_mapping;
   a.cu_rows = rows_of_seg ? (const int*)x.cu_rows : nullptr; a.seg_start = (const int*)x.seg_start; a.part = part; a.counters = (unsigned*)x.counters;
   a.sinks = (const float*)x.sinks; a.slopes = (const float*)x.slopes; a.rates = (const float*)x.rates;
-  a.n_rows = n_rows; a.ld = ld; a.out_ld = (int)x.out_ld; a.k_off = (int)x.k_off; a.v_off = (int)x.v_off; a.max_blocks = max_blocks; a.num_pages = num_pages; a.n_seqs = n_seqs;
+  a.n_rows = n_rows; a.ld = ld; a.out_ld = (int)x.out_ld; a.k_off = q8_int(x.k_off); a.v_off = q8_int(x.v_off); a.max_blocks = max_blocks; a.num_pages = num_pages; a.n_seqs = n_seqs;
   a.seg0 = seg0; a.n_items = (int)p.items; a.tiles_per_seg = p.tiles_per_seg; a.n_head = n_head; a.n_kv_head = n_kv_head;
   a.heads_per = p.heads_per; a.head_blocks = p.head_blocks; a.rows_per = p.rows_per;
   a.stages = p.stages; a.join_cols = p.join_cols; a.page_rows = n_kv_head * ps; a.hd = hd; a.ps = ps; a.ps_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (ps == 1 << i) a.ps_shift = i;
-  a.window = window; a.keep = keep; a.temp_every = (int)x.temp_every; a.scale = (float)x.scale; a.cap = (float)x.cap;
+  a.window = window; a.keep = keep; a.temp_every = q8_int(x.temp_every); a.scale = (float)x.scale; a.cap = (float)x.cap;
   a.temp_coef = (float)x.temp_coef;
   const bool ext = a.cap > 0.f || (keep > 0 && window != 0) || a.slopes || a.temp_every > 0;
   cudaStream_t st = (cudaStream_t)x.stream;

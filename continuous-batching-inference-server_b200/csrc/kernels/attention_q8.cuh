@@ -7,14 +7,17 @@
 //   * scores: mma.sync on signed bytes, keys as they lie in memory.  A query's numbers become whole numbers below 2^22 times a power of
 //     two of its own, cut into three signed bytes each, so the products are exact and a number is off by 2^-23 of the query's
 //     largest at most, for bfloat16 and for 32-bit rows alike;
-//   * values: mma.sync on bfloat16, which holds a code exactly, with the weights times vs_j rounded to bfloat16 (half a step, 2^-8, as the
-//     other attention kernels round theirs), or in three bfloat16 parts for 32-bit rows.
+//   * values: mma.sync on bfloat16, which holds a code exactly, with the weights times vs_j cut into two bfloat16 parts for bfloat16 rows
+//     (an error of 2^-17: one part costs 2^-9 of the result's size against 64 bits, as much as the rounding of the result itself) and
+//     into three for 32-bit rows.
 //
 // Both products are taken with the operands swapped, keys and values as the 16-row operand and the queries as the 8 columns:
 // S^T = K Q^T, O^T = V^T P^T.  The query heads that share a key/value head, and a chunk's rows, are the columns, so up to 8 of them cost
-// what one does.  The order of the contraction, and that of the output's rows, is free: a lane's share of the values is 16-byte pieces of its four keys.  They come through shared memory, a ring of stages for every warp alone, which it fills with
-// 16-byte asynchronous copies and reads without two lanes on one bank (q8_place): what is on its way holds no registers, so four
-// blocks fit on an SM, and a block asks for the first tiles of its next piece before it finishes the one in hand.
+// what one does (16 take a second set of columns; more were slower everywhere).  The order of the contraction, and that of the output's
+// rows, is free: a lane's share of the values is 16-byte pieces of its four keys.  They come through shared memory, a ring of stages for
+// every warp alone, which it fills with 16-byte asynchronous copies and reads without two lanes on one bank (q8_place): what is on its
+// way holds no registers, so three or four blocks fit on an SM, and a block asks for the first tiles of its next piece before it finishes
+// the one in hand.
 //
 // The tiles of 16 keys of all (row, head) pairs, and for every pair a few more for what it costs beside them, are one row that is cut
 // evenly over the blocks: every block works out its part from the positions on the device.  A cut that would leave a short end of a
@@ -171,7 +174,7 @@ struct Q8Place {
   }
 };
 
-// HDP: the width rounded up to 32, 64, 128 or 256; NT: columns of queries / 8; PARTS: bfloat16 parts of a weight (1: bfloat16 rows, 3:
+// HDP: the width rounded up to 32, 64, 128 or 256; NT: columns of queries / 8; PARTS: bfloat16 parts of a weight (2: bfloat16 rows, 3:
 // 32-bit rows); EXT: kept first keys, a cap, a distance bias, a query temperature; FAST: the width is HDP and pages are a multiple of 16 keys.
 template <int HDP, int NT, int PARTS>
 struct Q8Shape {
@@ -196,7 +199,7 @@ __host__ __device__ inline Q8Smem q8_smem(int stage, int lds, int ldq, int stage
   s.stats = s.join + (Q8_WARPS * jq * lds * 4 > 2048 ? Q8_WARPS * jq * lds * 4 : 2048);      // (2 KB: the groups' sums of a merge)
   s.queries = s.stats + Q8_WARPS * 8 * 2 * 4;
   s.columns = s.queries + 3 * live * ldq;
-  s.ints = s.columns + 3 * 32 * 4;
+  s.ints = s.columns + 3 * 16 * 4;
   s.items = s.ints + 32;
   s.bytes = s.items + (4 * n_items + 1) * 4;
   return s;
@@ -217,8 +220,8 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
   float* sm_m = reinterpret_cast<float*>(smem + at.stats);           // [warp][8]
   float* sm_l = sm_m + Q8_WARPS * 8;                                 // [warp][8]
   int8_t* sm_q = reinterpret_cast<int8_t*>(smem + at.queries);       // [3][cols][LDQ] the queries' bytes, the highest first
-  float* sm_f = reinterpret_cast<float*>(smem + at.columns);         // [32] a query's power of two, [32] maximum and [32] sum of merged pieces
-  float* sm_w = sm_f + 32;
+  float* sm_f = reinterpret_cast<float*>(smem + at.columns);         // [16] a query's power of two, [16] maximum and [16] sum of merged pieces
+  float* sm_w = sm_f + 16;
   int* sm_i = reinterpret_cast<int*>(smem + at.ints);                // [8]
   int* before = reinterpret_cast<int*>(smem + at.items);             // [n_items + 1] tiles of the items before this one
   int* item_row = before + a.n_items + 1;                            // [n_items] first row; request or rows; first position
@@ -264,10 +267,10 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
   __syncthreads();
   const int n_hg = a.n_kv_head * a.head_blocks, group = a.n_head / a.n_kv_head;
   if (total == 0) return;
-  // at least two rounds of the warps to a block; cuts are moved by up to three rounds (a merge takes about as long), by less where a block
-  // has much to do, for all wait for the one that got more
-  const long long all = (long long)total * n_hg, per = max((all + gridDim.x - 1) / gridDim.x, 2LL * UNIT);
-  const int slack = (int)min(per <= 6 * UNIT ? per - 1 : max(per / 16, (long long)Q8_PAIR), 3LL * UNIT);
+  // At least a round of the warps to a block (16 heads of 1,100 keys: 10.3 us with one, 12.7 with two, 15.0 with three); cuts are moved by
+  // up to three rounds (a merge takes about as long), by less where a block has much to do, for all wait for the one that got more.
+  const long long all = (long long)total * n_hg, per = max((all + gridDim.x - 1) / gridDim.x, (long long)(UNIT > Q8_PAIR + 1 ? UNIT : Q8_PAIR + 2));
+  const int slack = (int)min(per <= 6 * UNIT ? per - 1 : max(per / 16, (long long)Q8_PAIR), max(3LL * UNIT, (long long)Q8_PAIR));
   // the item in which tile `rem` of a head lies: the last one that begins at or before it
   auto item_at = [&](int rem) {
     int lo = 0, hi = a.n_items - 1;
@@ -435,7 +438,7 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
   while (true) {
     const int live = cur.it.n_rows * cur.n_h, n_h = cur.n_h;
     const int n_h_inv = (65536 + n_h - 1) / n_h;
-    auto row_in = [&](int m) { return m * n_h_inv >> 16; };      // m / n_h, exact for m and n_h up to 32
+    auto row_in = [&](int m) { return m * n_h_inv >> 16; };      // m / n_h, exact for m and n_h up to 16
     // queries as three signed bytes a number, a warp to a query
     for (int m = warp; m < live; m += Q8_WARPS) {
       float x[HDP / 32];
@@ -683,9 +686,19 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
             const unsigned A[4] = {q8_pair(__byte_perm(vw[0][w], vw[1][w], lo), base), q8_pair(__byte_perm(vw[0][w], vw[1][w], hi), base),
                                    q8_pair(__byte_perm(vw[2][w], vw[3][w], lo), base), q8_pair(__byte_perm(vw[2][w], vw[3][w], hi), base)};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+              float (&sum)[4] = o[nt][2 * w0 + j];
+              if constexpr (PARTS == 3) {      // the tensor cores cut their sums instead of rounding them: 32-bit rows add the tiles' own sums
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int p = PARTS - 1; p >= 0; --p) mma_16816(o[nt][2 * w0 + j], A, pf[p][nt][0], pf[p][nt][1]);
+                for (int p = PARTS - 1; p >= 0; --p) mma_16816(part, A, pf[p][nt][0], pf[p][nt][1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] += part[e];
+              } else {
+#pragma unroll
+                for (int p = PARTS - 1; p >= 0; --p) mma_16816(sum, A, pf[p][nt][0], pf[p][nt][1]);
+              }
+            }
           }
         }
       }
@@ -793,7 +806,7 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
           l = warp_sum(l * ex2(M - r)) + (a.sinks ? ex2(sk - r) : 0.f);
           if (lane == 0) {
             sm_w[m] = r;
-            sm_w[32 + m] = l;
+            sm_w[16 + m] = l;
           }
         }
         __syncthreads();
@@ -839,7 +852,7 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
             }
           }
           if (part < groups) {
-            const float l = sm_w[32 + m];
+            const float l = sm_w[16 + m];
             const int h = done.h0 + m - row_in(m) * n_h;
             TT* out = static_cast<TT*>(a.out) + (size_t)(done.it.row0 + row_in(m)) * a.out_ld + h * hd;
 #pragma unroll

@@ -224,9 +224,9 @@ CBIS_EXPORT int cbis_kv_write_q8(const void* call) {
   void *kc = (void*)x.kc, *ks = (void*)x.ks, *vc = (void*)x.vc, *vs = (void*)x.vs, *stream = (void*)x.stream;
   const int* slot_mapping = (const int*)x.slot_mapping;
   int hd_v = (int)x.hd_v;
-  const int ld = (int)x.ld, k_off = (int)x.k_off, v_off = (int)x.v_off, T = (int)x.T, heads = (int)x.heads, hd = (int)x.hd, ps = (int)x.ps,
-            dtype = (int)x.dtype;
-  if (x.n_slots > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
+  const int ld = (int)x.ld, k_off = q8_int(x.k_off), v_off = q8_int(x.v_off), T = q8_int(x.T), heads = q8_int(x.heads), hd = q8_int(x.hd),
+            ps = q8_int(x.ps), dtype = (int)x.dtype;
+  if (x.n_slots > 0x7fffffffLL || x.ld > 0x7fffffffLL) return CBIS_ERR_TOO_LARGE;
   const int n_slots = (int)x.n_slots;
   if (T <= 0) return CBIS_OK;
   if (hd_v <= 0) hd_v = hd;
@@ -283,8 +283,8 @@ CBIS_EXPORT int cbis_kv_read_q8(const void* call) {
   void *ko = (void*)x.ko, *vo = (void*)x.vo, *stream = (void*)x.stream;
   const int *block_table = (const int*)x.block_table, *seg_start = (const int*)x.seg_start, *seg_ctx = (const int*)x.seg_ctx;
   int hd_v = (int)x.hd_v;
-  const int max_blocks = (int)x.max_blocks, num_pages = (int)x.num_pages, n_seg = (int)x.n_seg, max_tokens = (int)x.max_tokens, heads = (int)x.heads,
-            hd = (int)x.hd, ps = (int)x.ps, window = (int)x.window, keep = (int)x.keep, whole = (int)x.flags & 1, dtype = (int)x.flags >> 1 & 1, as_codes = (int)x.flags >> 2;
+  const int max_blocks = q8_int(x.max_blocks), num_pages = q8_int(x.num_pages), n_seg = q8_int(x.n_seg), max_tokens = q8_int(x.max_tokens), heads = (int)x.heads,
+            hd = (int)x.hd, ps = (int)x.ps, window = q8_int(x.window), keep = q8_int(x.keep), whole = (int)x.flags & 1, dtype = (int)x.flags >> 1 & 1, as_codes = (int)x.flags >> 2;
   if (n_seg <= 0 || max_tokens <= 0) return CBIS_OK;
   if (hd_v <= 0) hd_v = hd;
   if (heads <= 0 || hd <= 0 || ps <= 0 || max_blocks <= 0 || keep < 0 || n_seg > 65535) return CBIS_ERR_BAD_SIZE;

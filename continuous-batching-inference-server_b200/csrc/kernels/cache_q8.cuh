@@ -10,6 +10,12 @@
 
 namespace cbis {
 
+// A number of a call's record as an int: what lies beyond 2^30 (behind every position) is 2^30 + 1, below -2^30 it is -2^30 - 1.
+inline int q8_int(long long x) {
+  const long long most = (1 << 30) + 1;
+  return (int)(x > most ? most : (x < -most ? -most : x));
+}
+
 constexpr float Q8_FLOOR = 7.52316384526264e-37f;      // 2^-120
 
 // The largest magnitude as the bits of |x|: ordered like the magnitudes, an infinity above every number and a NaN above that.

@@ -179,7 +179,7 @@ def _coded(ctx, mixer, qkv, cache, view, out, gate) -> int:
     extra.update(cap=float(getattr(mixer, "cap", 0.0)), keep=int(getattr(mixer, "keep_first", 0)))
     if (not one and getattr(mixer, "talk", None) is None and ops.attention_q8_takes(hd, vd) and qkv.stride(0) % per == 0
             and qkv.data_ptr() % 16 == 0 and nd <= ops.ATTENTION_Q8_MAX_ROWS
-            and (T == nd or ops.prefill_q8_takes(T - nd, ctx.max_seg_rows, ctx.n_segments - nd, ctx.ctx_limit, H, G, hd, ps, qkv.dtype, **extra))):
+            and (T == nd or ops.prefill_q8_takes(T - nd, ctx.max_seg_rows, ctx.n_segments - nd, H, G, hd, ps, qkv.dtype, **extra))):
         work, limit = (cache.values.arrays[k_name], cache.values.arrays[v_name]), ctx.ctx_limit
         if nd > 0:
             scratch = ctx.decode_scratch(*_coded_scratch(ctx, nd, 1, nd, H, G, hd, limit, qkv.dtype))

@@ -629,13 +629,14 @@ def _q8_table(what: str, block_table) -> None:
 
 def kv_write_q8(qkv, k_off, v_off, k_pages, v_pages, slot_mapping, n_kv_head, head_dim, page_size, v_head_dim=0):
     """``kv_write`` into an 8-bit cache: rows of this step's K and V (columns k_off.. and v_off.. of qkv, bfloat16 or float32) are
-    quantised, a scale per token and head, and go to their token slots (a slot that the cache does not have writes nothing).
+    quantised, a scale per token and head, and go to their token slots, which are different ones (a slot that the cache does not have
+    writes nothing).
     ``v_head_dim``: the values' width where it is not the keys'.  ``v_pages`` None, or the keys' own pages: one array stands for
     both and takes the rows at k_off."""
     what = "kv_write_q8"
     vd = int(v_head_dim) or head_dim
     kc, ks = k_pages
-    vc, vs = (None, None) if v_pages is None or v_pages[0] is kc else v_pages
+    vc, vs = (None, None) if v_pages is None or v_pages[0].data_ptr() == kc.data_ptr() else v_pages
     T = qkv.shape[0]
     code = dtype_code(qkv.dtype)
     shape, dev, columns = kc.shape, qkv.get_device(), qkv.shape[-1]
@@ -671,7 +672,7 @@ def kv_read_q8(k_pages, v_pages, k_out, v_out, block_table, seg_start, seg_ctx, 
     ``v_out`` through the same block table.  ``v_pages`` None: one array."""
     what = "kv_read_q8"
     kc, ks = k_pages
-    vc, vs = (None, None) if v_pages is None or v_pages[0] is kc else v_pages
+    vc, vs = (None, None) if v_pages is None or v_pages[0].data_ptr() == kc.data_ptr() else v_pages
     code = dtype_code(k_out.dtype)
     shape, dev = kc.shape, kc.get_device()
     S = block_table.shape[0]
@@ -732,7 +733,8 @@ def _q8_scratch(n, rows_of_seg, n_head, n_kv_head, head_dim, code, max_context):
 
 def attention_q8_scratch(rows: int, max_seg_rows: int, n_seg: int, n_head: int, n_kv_head: int, head_dim: int, max_context: int, dtype):
     """(floats, int32 counters) that ``paged_decode_q8`` over ``rows`` rows and ``paged_prefill_q8`` over ``n_seg`` requests of ``rows``
-    rows in all, at most ``max_seg_rows`` each, need; the counters are zero before the first launch, and every launch leaves them zero."""
+    rows in all, at most ``max_seg_rows`` each, need; the counters are zero before the first launch, and every launch leaves them zero.  Launches that may run at the same time
+    need scratch and counters of their own."""
     code = dtype_code(dtype)
     if max_seg_rows <= 1:
         st, floats, counters = _q8_scratch(max(rows, n_seg), 0, n_head, n_kv_head, head_dim, code, max_context)
@@ -746,10 +748,16 @@ def attention_q8_scratch(rows: int, max_seg_rows: int, n_seg: int, n_head: int, 
 
 
 def _prefill_q8_chunks(max_seg_rows, n_seg, n_head, head_dim, max_context, dtype):
-    """The key chunks of the kernel that attends to the values read back."""
-    if dtype == torch.bfloat16 and head_dim in (64, 128) and USE_TCGEN05:
-        return prefill_key_chunks(-(-max_seg_rows // 128), n_head, n_seg, max_context, 2, 2, 8192)
-    return prefill_key_chunks(-(-max_seg_rows // 64), n_head, n_seg, max_context, 1, 8 if dtype == torch.bfloat16 else 16)
+    """(n_chunks, chunk_keys) of the kernel that attends to the values read back.  The tcgen05 kernel's blocks, two a row tile, are cut into
+    equal parts that fill the SMs (two blocks each) once, of at least 1,000 keys: 512 rows of 16 heads of 128 behind 8,192 tokens 114 us
+    whole, 79 in two parts of 4,352 keys, 126 in 8,192 and the rest; 128 rows behind 7,872 83 us whole, 38 in eight parts."""
+    if dtype == torch.bfloat16:
+        n = min(296 // max(1, -(-max_seg_rows // 128) * 2 * n_head * n_seg), max_context // 1000) if USE_KEY_CHUNKS else 1
+        if n < 2:
+            return 1, 0
+        keys = -(-max_context // (64 * n)) * 64
+        return -(-max_context // keys), keys
+    return prefill_key_chunks(-(-max_seg_rows // 64), n_head, n_seg, max_context, 1, 16)
 
 
 def _q8_attention_ok(q, kc, ks, vc, vs, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, slopes, sinks, rates, keep) -> bool:
@@ -807,7 +815,8 @@ def paged_decode_q8(qkv, k_off, v_off, k_pages, v_pages, block_table, row_seq, p
                     n_kv_head, head_dim, page_size, scale, window, max_context, slopes=None, sinks=None, q_temp=None, rates=None,
                     cap: float = 0.0, keep: int = 0):
     """Decode attention (one query per row, bfloat16 or float32) over an 8-bit cache; with ``k_off >= 0`` the current token's key and
-    value are taken from ``qkv``, quantised and stored by the same kernel.  No context is longer than ``max_context``.  Head sizes
+    value are taken from ``qkv``, quantised and stored by the same kernel; the rows are then of different requests (two new tokens of one
+    are a chunk).  No context is longer than ``max_context``.  Head sizes
     that are multiples of 16 up to 256, any page size.  ``scratch``, ``counters``: ``attention_q8_scratch``.  ``window``, ``slopes``, ``sinks``,
     ``q_temp``, ``rates``, ``cap``, ``keep``: as in ``paged_attention_generic``.  A row whose request is no row of the block table, or that sees no
     key, gets zeros; a page number that the cache does not have is passed over."""
@@ -820,7 +829,7 @@ def paged_decode_q8(qkv, k_off, v_off, k_pages, v_pages, block_table, row_seq, p
                                           slopes, sinks, rates, keep)
             and row_seq.dtype is _INT32 and positions.dtype is _INT32 and row_seq.is_contiguous() and positions.is_contiguous()
             and row_seq.numel() >= rows and positions.numel() >= rows and qkv.get_device() == row_seq.get_device() == positions.get_device()
-            and (k_off < 0 or (v_off >= 0 and max(k_off, v_off) + n_kv_head * head_dim <= qkv.shape[1] and slot_mapping is not None
+            and (k_off < 0 or (v_off >= 0 and kc.data_ptr() != vc.data_ptr() and max(k_off, v_off) + n_kv_head * head_dim <= qkv.shape[1] and slot_mapping is not None
                                and slot_mapping.dtype is _INT32 and slot_mapping.is_contiguous() and slot_mapping.numel() >= rows
                                and slot_mapping.get_device() == qkv.get_device()))):
         _q8_attention_checks(what, qkv, k_pages, v_pages, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, slopes,
@@ -829,6 +838,7 @@ def paged_decode_q8(qkv, k_off, v_off, k_pages, v_pages, block_table, row_seq, p
         _q8_int32(what, "positions", positions, rows)
         if k_off >= 0:
             wide = n_kv_head * head_dim
+            _q8_need(rows == 0 or kc.data_ptr() != vc.data_ptr(), what, "keys and values of one array cannot both be stored")
             _q8_need(v_off >= 0 and max(k_off, v_off) + wide <= qkv.shape[1], what, f"keys and values of {wide} do not lie in rows of {tuple(qkv.shape)}")
             _q8_int32(what, "slot_mapping", slot_mapping, rows)
         _q8_here(what, qkv, kc, ks, vc, vs, block_table, row_seq, positions, slot_mapping if k_off >= 0 else None, out, scratch, counters,
@@ -840,16 +850,17 @@ def paged_decode_q8(qkv, k_off, v_off, k_pages, v_pages, block_table, row_seq, p
                   sinks, q_temp, rates, float(cap), int(keep))
 
 
-def prefill_q8_reads_back(n_rows: int, max_seg_rows: int, n_seg: int, keys: int, n_head: int, n_kv_head: int, head_dim: int, page_size: int, dtype,
+def prefill_q8_reads_back(n_rows: int, max_seg_rows: int, n_seg: int, n_head: int, n_kv_head: int, head_dim: int, page_size: int, dtype,
                           slopes=None, sinks=None, q_temp=None, rates=None, cap: float = 0.0, keep: int = 0) -> bool:
-    """Whether ``paged_prefill_q8`` reads the cache back first (no row sees more than ``keys`` keys): where the kernel over pages of q's type
-    is faster, or the one that reads codes cannot count the row tiles.
+    """Whether ``paged_prefill_q8`` reads the cache back first: where the kernel over pages of q's type is faster, or the one that reads
+    codes cannot count the row tiles.
 
-    In bfloat16 that is the tcgen05 kernel over codes as they are.  Against the kernel that reads codes it saves some 3.5 us a million
-    pairs of row and key (times heads, of 128), and costs some 8 us more, and 1 us a million numbers read back.  16 heads of 128 behind 2,000 keys:
-    32 rows 24.2 us here and 34.2 there, 64 rows 32.0 and 34.2, 128 rows 39.9 and 34.4, 512 rows behind 8,192 268 and 148; twelve requests
-    of 16 rows behind 1,000 keys 43.9 and 69.1, over 4 key/value heads 43.9 and 47.2.  In 32 bits the kernel that reads codes multiplies
-    on the tensor cores and is the faster one: 512 rows of 8 heads of 32 behind 8,192 85 us and 131, 256 rows of 16 heads over 4 of 64 behind 2,000
+    In bfloat16 that is the tcgen05 kernel over codes as they are.  For every thousand keys it takes some 0.12 us a tile of 128 rows and head
+    (0.08 at head size 64), however few of the rows there are, and reading back 0.0011 us a number of a token; the kernel that
+    reads codes takes 0.004 us a row and head of 128.  16 heads of 128 behind 2,000 keys: 32 rows 25.1 us here and 29.5 there, 64 rows
+    32.7 and 29.9, 128 rows 41.7 and 31.3, 512 rows behind 8,192 294 and 102; twelve requests of 16 rows behind 1,000 keys 45.2 and 69.0,
+    over 4 key/value heads 45.2 and 47.6, of 32 heads over 4 of 64 41.7 and 64.8.  In 32 bits the kernel that reads codes multiplies on the
+    tensor cores and is the faster one: 512 rows of 8 heads of 32 behind 8,192 85 us and 131, 256 rows of 16 heads over 4 of 64 behind 2,000
     43 and 75."""
     wide = dtype == torch.float32
     if page_size & (page_size - 1) or slopes is not None or q_temp is not None or (
@@ -858,12 +869,13 @@ def prefill_q8_reads_back(n_rows: int, max_seg_rows: int, n_seg: int, keys: int,
     group = n_head // n_kv_head
     if n_seg * -(-max_seg_rows // max(1, 16 // group)) > ATTENTION_Q8_MAX_ROWS:
         return True
-    return not wide and 3.5e-6 / 128 * n_rows * n_head * keys * head_dim > 8 + 1e-6 * n_seg * keys * n_kv_head * head_dim
+    tiles = n_seg * -(-max_seg_rows // 128) * n_head
+    return not wide and 0.004 / 128 * n_rows * n_head * head_dim > (0.12 if head_dim == 128 else 0.08) * tiles + 0.0011 * n_seg * n_kv_head * head_dim
 
 
-def prefill_q8_takes(n_rows: int, max_seg_rows: int, n_seg: int, keys: int, n_head: int, n_kv_head: int, head_dim: int, page_size: int, dtype, **extra) -> bool:
+def prefill_q8_takes(n_rows: int, max_seg_rows: int, n_seg: int, n_head: int, n_kv_head: int, head_dim: int, page_size: int, dtype, **extra) -> bool:
     """Whether ``paged_prefill_q8`` with ``work`` takes these sizes (the kernel that reads codes counts its row tiles)."""
-    return (prefill_q8_reads_back(n_rows, max_seg_rows, n_seg, keys, n_head, n_kv_head, head_dim, page_size, dtype, **extra)
+    return (prefill_q8_reads_back(n_rows, max_seg_rows, n_seg, n_head, n_kv_head, head_dim, page_size, dtype, **extra)
             or _q8_scratch(n_seg, max_seg_rows, n_head, n_kv_head, head_dim, dtype_code(dtype), 1)[0] == 0)
 
 
@@ -906,17 +918,22 @@ def paged_prefill_q8(q, k_pages, v_pages, block_table, cu_rows, seg_start, seg_c
     if n_seg == 0 or n_rows == 0 or max_seg_rows <= 0:
         return
     window, cap, keep = int(window), float(cap), int(keep)
-    tokens = min(max_context, abs(window) + max_seg_rows) if window else max_context
     if work is None or out.data_ptr() % 16 or out.stride(0) % 8 or not prefill_q8_reads_back(
-            n_rows, max_seg_rows, n_seg, tokens, n_head, n_kv_head, head_dim, page_size, q.dtype, slopes, sinks, q_temp, rates, cap, keep):
+            n_rows, max_seg_rows, n_seg, n_head, n_kv_head, head_dim, page_size, q.dtype, slopes, sinks, q_temp, rates, cap, keep):
         return _attention_q8(what, q, -1, -1, k_pages, v_pages, block_table, None, None, None, cu_rows, seg_start, seg0, n_seg,
                              int(max_seg_rows), out, scratch, counters, n_head, n_kv_head, head_dim, page_size, scale, window,
                              int(max_context), slopes, sinks, q_temp, rates, cap, keep)
+    far = 2 ** 30 + 1       # behind every position
+    window, keep, max_context = max(-far, min(window, far)), min(keep, far), min(int(max_context), far)
     k, v = work
+    tokens = min(max_context, abs(window) + max_seg_rows) if window else max_context
     blocks, wide = block_table.shape[1], q.dtype is _FLOAT32
+    # (behind a window most parts would be empty)
+    chunks = (1, 0) if window and not wide else _prefill_q8_chunks(max_seg_rows, n_seg, n_head, head_dim, max_context, q.dtype)
+    need = n_rows * n_head * chunks[0] * (head_dim + 4) if chunks[0] > 1 else 0
+    _q8_need(scratch.numel() >= need, what, f"scratch has {scratch.numel()} numbers and not {need}")
     _kv_read_q8(kc, ks, vc, vs, k, v, block_table.data_ptr() + 4 * seg0 * blocks, blocks, seg_start.data_ptr() + 4 * seg0,
                 seg_ctx.data_ptr() + 4 * seg0, n_seg, tokens, window, keep, 1 | (F32 if wide else BF16) << 1 | (not wide) << 2)
-    chunks = _prefill_q8_chunks(max_seg_rows, n_seg, n_head, head_dim, max_context, q.dtype)
     args = (q, k, v, block_table, cu_rows, seg_start, out, seg0, n_seg, max_seg_rows, n_head, n_kv_head, head_dim, page_size, scale, window)
     if wide:
         return paged_prefill_f32(*args, chunks, scratch, positions, row0, n_rows)

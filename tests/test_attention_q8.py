@@ -168,7 +168,7 @@ def prefill(ops, c, window=0, work=False, seg0=0, out=None, max_context=None, **
     pages = tuple(torch.full(c["k"].codes.shape, math.nan, dtype=c["dtype"], device="cuda") for _ in "kv") if work else None
     takes = ops.prefill_q8_reads_back
     if work:        # wherever there is a kernel over pages read back, whichever is the faster one
-        ops.prefill_q8_reads_back = lambda rows, most, n_seg, keys, *rest: takes(10 ** 9, most, n_seg, keys, *rest) or takes(rows, 10 ** 9, n_seg, keys, *rest)
+        ops.prefill_q8_reads_back = lambda rows, most, n_seg, *rest: takes(10 ** 9, most, n_seg, *rest) or takes(rows, 10 ** 9, n_seg, *rest)
     start = torch.tensor([a - b for a, b in zip(c["ctx"], c["rows"])], dtype=torch.int32).cuda()
     ops.paged_prefill_q8(c["q"].cuda(), c["k"], c["v"], c["table"].cuda(), c["cu"].cuda(), start, torch.tensor(c["ctx"], dtype=torch.int32).cuda(),
                          c["positions"].cuda(), out, seg0, n, row0, rows, max(c["rows"]), c["H"], c["G"], c["hd"], c["ps"], c["hd"] ** -0.5, window,
@@ -180,7 +180,7 @@ def prefill(ops, c, window=0, work=False, seg0=0, out=None, max_context=None, **
 
 def test_which_kernel_takes_a_chunk():
     from cbis_b200.kernels import ops
-    small = dict(n_seg=1, keys=2000, n_head=16, n_kv_head=16, head_dim=128, page_size=16, dtype=BF)
+    small = dict(n_seg=1, n_head=16, n_kv_head=16, head_dim=128, page_size=16, dtype=BF)
     reads = lambda rows, **kw: ops.prefill_q8_reads_back(rows, rows, **{**small, **kw})      # noqa: E731
     assert not reads(32) and reads(256) and not reads(256, head_dim=96) and not reads(256, page_size=24) and not reads(256, q_temp=(0.1, 5))
     assert not reads(256, slopes=1, rates=1) and reads(256, sinks=1) and reads(256, cap=3.0, keep=2)
@@ -440,3 +440,83 @@ def test_refusals_of_the_launcher(ops):
         big = torch.zeros(5000, 64, dtype=BF, device="cuda")
         decode(ops, dict(c, positions=torch.zeros(5000, dtype=torch.int32)), q=big, seq=torch.zeros(5000, dtype=torch.int32),
                buffers=(torch.zeros(1 << 22, device="cuda"), torch.zeros(1 << 15, dtype=torch.int32, device="cuda")))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_numbers_behind_every_position(ops, dtype):
+    """A window, kept keys and a context that no position reaches, beyond 32 bits too, are those of a call without a limit."""
+    c = make(ops, dtype, 2, 2, 32, 16, [90, 33], [1, 1], seed=2)
+    plain = decode(ops, c)
+    for far in (2 ** 30, 2 ** 31 + 5, 2 ** 32 + 40):
+        assert torch.equal(decode(ops, c, far), plain)
+        assert torch.equal(decode(ops, c, 0, max_context=90, buffers=scratch(ops, 2, 1, 0, c), keep=far), plain)
+        # (kept first keys are seen by every row: the window's start is then no limit)
+        check(c, decode(ops, c, 20, keep=far), 32 ** -0.5, 20, 90)
+    with pytest.raises(ops.KernelError, match="a size"):
+        decode(ops, c, -2 ** 31)
+    c = make(ops, dtype, 2, 2, 64, 16, [190, 130], [150, 90], seed=2)
+    for far in (2 ** 30, 2 ** 31 + 5, 2 ** 32 + 40):
+        check(c, prefill(ops, c, far), 1 / 8, rows=[0, 149, 150, 239])
+        if dtype == BF:
+            check(c, prefill(ops, c, far, work=True, keep=far), 1 / 8, rows=[0, 149, 150, 239])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_page_that_the_cache_does_not_have_in_a_long_chunk(ops, hd):
+    """Over pages read back such a page holds nothing: the rows that see it get not-a-numbers, the others their results."""
+    for page in (-1, 10 ** 6):
+        c = make(ops, BF, 4, 2, hd, 16, [300, 260], [150, 140], seed=9)
+        c["table"][0, 200 // 16] = page
+        out = prefill(ops, c, work=True)
+        for r in range(290):
+            hit = r < 150 and 150 + r >= 192
+            assert torch.isnan(out[r].float()).all().item() == hit, r
+        check(c, out, hd ** -0.5, rows=[0, 41, 150, 200, 289])
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once(ops):
+    """On two streams, each with scratch and counters of its own."""
+    cs = [make(ops, BF, 8, 2, 128, 16, [3000, 40, 1777], [1, 1, 1], seed=s) for s in (7, 8)]
+    alone = [decode(ops, c) for c in cs]
+    fixed = [(c["q"].cuda(), c["table"].cuda(), c["seq"].cuda(), c["positions"].cuda(), torch.zeros_like(alone[0]), scratch(ops, 3, 1, 0, c)) for c in cs]
+    streams = [torch.cuda.Stream() for _ in cs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for c, (q, table, seq, pos, out, buf), stream in zip(cs, fixed, streams):
+            with torch.cuda.stream(stream):
+                ops.paged_decode_q8(q, -1, -1, c["k"], c["v"], table, seq, pos, None, out, *buf, 8, 2, 128, 16, 128 ** -0.5, 0, 3000)
+    torch.cuda.synchronize()
+    for (_, _, _, _, out, _), ref in zip(fixed, alone):
+        assert torch.equal(out, ref)
+
+
+@pytest.mark.gpu
+def test_scratch_of_a_long_chunk(ops):
+    """The parts of a long context need room: less is refused before anything is launched."""
+    c = make(ops, BF, 2, 1, 128, 16, [9000], [70], seed=3)
+    work = tuple(torch.zeros(c["k"].codes.shape, dtype=BF, device="cuda") for _ in "kv")
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")      # noqa: E731
+    out = torch.full(c["q"].shape, 7.5, dtype=BF, device="cuda")
+    floats, counters = ops.attention_q8_scratch(70, 70, 1, 2, 1, 128, 9000, BF)
+    takes, ops.prefill_q8_reads_back = ops.prefill_q8_reads_back, lambda *a: True
+    try:
+        with pytest.raises(ops.KernelError, match="scratch has"):
+            ops.paged_prefill_q8(c["q"].cuda(), c["k"], c["v"], c["table"].cuda(), c["cu"].cuda(), i32(8930), i32(9000), c["positions"].cuda(), out, 0, 1, 0,
+                                 70, 70, 2, 1, 128, 16, 1.0, 0, 9000, torch.zeros(100, device="cuda"), torch.zeros(counters, dtype=torch.int32, device="cuda"), work)
+    finally:
+        ops.prefill_q8_reads_back = takes
+    assert torch.all(out == 7.5) and not any(w.any() for w in work)
+
+
+def test_one_array_is_not_stored_twice():
+    """Both of a token's rows would go to one place."""
+    from cbis_b200.kernels import ops
+    p = ops.q8_pages(2, 2, 16, 32, device="cpu")
+    q, out = torch.zeros(3, 256, dtype=BF), torch.zeros(3, 128, dtype=BF)
+    i, table, f = torch.zeros(4, dtype=torch.int32), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(1 << 16)
+    for v in (p, ops.Q8Pages(p.codes.view(p.codes.shape), p.scales)):
+        with pytest.raises(ops.KernelError, match="of one array"):
+            ops.paged_decode_q8(q, 128, 192, p, v, table, i, i, i, out, f, i, 4, 2, 32, 16, 1.0, 0, 32)
