@@ -113,12 +113,13 @@ CBIS_EXPORT int cbis_attention_q8(const void* call) {
   a.sinks = (const float*)x.sinks; a.slopes = (const float*)x.slopes; a.rates = (const float*)x.rates;
   a.n_rows = n_rows; a.ld = ld; a.out_ld = (int)x.out_ld; a.k_off = q8_int(x.k_off); a.v_off = q8_int(x.v_off); a.max_blocks = max_blocks; a.num_pages = num_pages; a.n_seqs = n_seqs;
   a.seg0 = seg0; a.n_items = (int)p.items; a.tiles_per_seg = p.tiles_per_seg; a.n_head = n_head; a.n_kv_head = n_kv_head;
-  a.heads_per = p.heads_per; a.head_blocks = p.head_blocks; a.rows_per = p.rows_per;
+  a.heads_per = p.heads_per; a.heads_inv = (65536 + p.heads_per - 1) / p.heads_per; a.head_blocks = p.head_blocks; a.rows_per = p.rows_per;
   a.stages = p.stages; a.join_cols = p.join_cols; a.page_rows = n_kv_head * ps; a.hd = hd; a.ps = ps; a.ps_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (ps == 1 << i) a.ps_shift = i;
   a.window = window; a.keep = keep; a.temp_every = q8_int(x.temp_every); a.scale = (float)x.scale; a.cap = (float)x.cap;
   a.temp_coef = (float)x.temp_coef;
+  a.grid_inv = p.blocks ? 1.000001f / (float)p.blocks : 0.f;
   const bool ext = a.cap > 0.f || (keep > 0 && window != 0) || a.slopes || a.temp_every > 0;
   cudaStream_t st = (cudaStream_t)x.stream;
   switch (p.hdp) {

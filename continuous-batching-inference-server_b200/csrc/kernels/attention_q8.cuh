@@ -22,6 +22,13 @@
 // The tiles of 16 keys of all (row, head) pairs, and for every pair a few more for what it costs beside them, are one row that is cut
 // evenly over the blocks: every block works out its part from the positions on the device.  A cut that would leave a short end of a
 // pair is moved to the pair's end: a pair that lies in several blocks is merged by the last one to finish it.
+//
+// Measured on one B200, in a graph (copies run at 6.45 TB/s): 64 rows of 120 to 1,400 keys under 16 heads of 128 50.6 us, 4.1 TB/s; 5 rows
+// of 7,000 to 30,011 keys, 16 heads over 4, 29.4 us, 3.1 TB/s (over a bfloat16 cache 59 and 71 us); one row of 1,100 keys, 16 heads,
+// 10.0 us, of which 2 go by before the first keys are asked for, 1.5 until they are there and 4 in the join, the ticket and the merge;
+// in 32 bits 16 rows of 300 to 2,000 keys, 8 heads of 32, 13.4 us; chunks of 2 to 7 rows of twelve requests, 25 heads of 64, 17.1 us.
+// A tile of a head takes some 450 warp instructions, 128 of them to make bfloat16 numbers of the values' codes; the schedulers are
+// busy 44 % of the time, with three warps each.
 #pragma once
 #include "cache_q8.cuh"
 #include "mma_sync.cuh"
@@ -46,7 +53,8 @@ struct Q8Args {
   const float *sinks, *slopes, *rates;
   int n_rows, ld, out_ld, k_off, v_off, max_blocks, num_pages, n_seqs, seg0, n_items, tiles_per_seg, n_head, n_kv_head, heads_per, head_blocks, rows_per;
   int stages, join_cols, page_rows, hd, ps, ps_shift, window, keep, temp_every;      // ps_shift: log2 of the page size, -1 where that is no whole number
-  float scale, cap, temp_coef;
+  int heads_inv;                  // ceil(2^16 / heads_per)
+  float scale, cap, temp_coef, grid_inv;
 };
 
 // Rows of one item: a decoding row, or some consecutive rows of a request's chunk.
@@ -157,6 +165,20 @@ __device__ __forceinline__ float read_float(unsigned at) {
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(at) : "memory");
   return r;
 }
+// floor(x / d) for x >= 0 and a quotient below 2^20, from the reciprocal inv of d (good to 2^-22, so the product is off by less than one): a
+// division takes some 200 cycles, and a block of few tiles forms five before it asks for its first key.
+__device__ __forceinline__ int quotient(long long x, long long d, float inv) {
+  int q = (int)((float)x * inv);
+  const long long r = x - (long long)q * d;
+  if (r < 0) --q;
+  if (r >= d) ++q;
+  return q;
+}
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 // The bytes 32 x .. 32 x + 31 of 16 keys as the A fragment of a product on signed bytes, from a lane's share of the addresses.
 __device__ __forceinline__ void read_keys(unsigned (&r)[4], unsigned at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -231,6 +253,8 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
   unsigned base;
   asm volatile("mov.b32 %0, 0x43004300;" : "=r"(base));
   pdl_trigger();
+  // the arguments' lines, and what does not depend on the kernels before, while those end
+  asm volatile("" ::"l"(a.q), "l"(a.block_table), "l"(a.part), "r"(a.n_rows), "r"(a.n_kv_head), "r"(a.hd), "f"(a.scale));
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
 
@@ -267,9 +291,10 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
   __syncthreads();
   const int n_hg = a.n_kv_head * a.head_blocks, group = a.n_head / a.n_kv_head;
   if (total == 0) return;
-  // At least a round of the warps to a block (16 heads of 1,100 keys: 10.3 us with one, 12.7 with two, 15.0 with three); cuts are moved by
+  // At least a round of the warps to a block (16 heads of 1,100 keys: 10.0 us with one, 12.5 with two, 15 with three); cuts are moved by
   // up to three rounds (a merge takes about as long), by less where a block has much to do, for all wait for the one that got more.
-  const long long all = (long long)total * n_hg, per = max((all + gridDim.x - 1) / gridDim.x, (long long)(UNIT > Q8_PAIR + 1 ? UNIT : Q8_PAIR + 2));
+  const long long all = (long long)total * n_hg, per = max((long long)((float)all * a.grid_inv) + 1, (long long)(UNIT > Q8_PAIR + 1 ? UNIT : Q8_PAIR + 2));      // (grid_inv is a little too large)
+  const float total_inv = reciprocal((float)total), per_inv = reciprocal((float)per);
   const int slack = (int)min(per <= 6 * UNIT ? per - 1 : max(per / 16, (long long)Q8_PAIR), max(3LL * UNIT, (long long)Q8_PAIR));
   // the item in which tile `rem` of a head lies: the last one that begins at or before it
   auto item_at = [&](int rem) {
@@ -282,13 +307,14 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
   };
   auto cut = [&](long long x) {      // a block's end, moved to that of an item that is near
     if (x >= all) return all;
-    const int rem = (int)(x % total), i = item_at(rem), d = rem - before[i], e = before[i + 1] - rem;
+    const int rem = (int)(x - (long long)quotient(x, total, total_inv) * total), i = item_at(rem), d = rem - before[i], e = before[i + 1] - rem;
     return d <= slack ? x - d : (e <= slack ? x + e : x);
   };
   long long w_at = cut(blockIdx.x * per);
   const long long w_end = cut((blockIdx.x + 1) * per);
   if (w_at >= w_end) return;
 
+  auto inverse = [&](int n_h) { return n_h == a.heads_per ? a.heads_inv : (65536 + n_h - 1) / n_h; };
   // A block's part of one item's keys under the heads that share a key/value head: from tile `from` to end_tile.
   struct Piece {
     Q8Item it;
@@ -299,7 +325,7 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
     const int8_t *k_lane, *v_lane;      // FAST: the lane's piece of the head's first row, and its scale
     const float* s_lane;
   };
-  int at_hg = (int)(w_at / total), at_item = item_at((int)(w_at % total)), at_tile = (int)(w_at % total) - before[at_item];
+  int at_hg = quotient(w_at, total, total_inv), at_item = item_at((int)(w_at - (long long)at_hg * total)), at_tile = (int)(w_at - (long long)at_hg * total) - before[at_item];
   auto find_piece = [&](Piece& p) {
     const int lo = at_item, slots = before[lo + 1] - before[lo], to = (int)min((long long)slots, at_tile + (w_end - w_at));
     p.hg = at_hg;
@@ -329,6 +355,11 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
     p.h0 = p.hk * group + hb * a.heads_per;
     p.n_h = min(a.heads_per, group - hb * a.heads_per);
     p.bt = a.block_table + (size_t)max(p.it.seq, 0) * a.max_blocks;
+    // the query that the warp converts first, on its way while the pages are looked up
+    if (lane * 128 < hd * (int)sizeof(TT) && warp < p.it.n_rows * p.n_h) {
+      const int row = inverse(p.n_h) * warp >> 16;
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const TT*>(a.q) + (size_t)(p.it.row0 + row) * a.ld + (p.h0 + warp - row * p.n_h) * hd + lane * (128 / (int)sizeof(TT))));
+    }
     if constexpr (FAST) {
       const long long first = (long long)p.hk * a.ps;
       p.k_lane = a.kc + first * HDP + lane * 16;
@@ -432,12 +463,14 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
     }
   };
 
+  int owed = 0;                            // 1: a ticket of the first piece, 2: of the last
+  unsigned ticket0 = 0, ticket1 = 0;       // of one thread
   Piece cur;
   find_piece(cur);
   ask_first(cur);
   while (true) {
     const int live = cur.it.n_rows * cur.n_h, n_h = cur.n_h;
-    const int n_h_inv = (65536 + n_h - 1) / n_h;
+    const int n_h_inv = inverse(n_h);
     auto row_in = [&](int m) { return m * n_h_inv >> 16; };      // m / n_h, exact for m and n_h up to 16
     // queries as three signed bytes a number, a warp to a query
     for (int m = warp; m < live; m += Q8_WARPS) {
@@ -777,93 +810,133 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
         }
       }
     }
+    // A piece of an item that others have a part of: a ticket is drawn now and looked at when the block is done with its last piece, so
+    // that nothing waits for it.  (Such are a block's first piece and its last; the barrier puts the block's stores before the fence.)
     if (!alone) {
-      // the cuts that were left inside the item; the piece behind cut c is block c's, the first piece that of the block before
-      const long long begin = (long long)done.hg * total + before[done.item], end = begin + before[done.item + 1] - before[done.item];
-      const int b_first = (int)((begin + slack) / per), n_pieces = (int)((end - slack - 1) / per) - b_first + 1;
       __syncthreads();
-      if (tid == 0) {      // (the barrier puts the block's stores before this thread's fence)
-        unsigned* counter = a.counters + (size_t)done.item * n_hg + done.hg;
+      owed |= more ? 1 : 2;
+      if (tid == Q8_THREADS - 32) {
+        sm_i[more ? 4 : 6] = done.item;
+        sm_i[more ? 5 : 7] = done.hg;
         __threadfence();
-        const bool last = atomicAdd(counter, 1u) == (unsigned)(n_pieces - 1);
-        sm_i[0] = last;
-        if (last) *counter = 0;
-        __threadfence();
-      }
-      __syncthreads();
-      if (sm_i[0]) {
-        auto piece = [&](int b) { return a.part + (size_t)(2 * (b_first + b) + (b == 0)) * NQ * (HDP + 4); };
-        // every column's maximum and denominator over the pieces first
-        for (int m = warp; m < live; m += Q8_WARPS) {
-          float M = -INFINITY, l = 0.f;
-          for (int b = lane; b < n_pieces; b += 32) {
-            const float* p = piece(b) + m * (HDP + 4) + HDP;
-            const float pm = load_float(p), pl = load_float(p + 1), top = fmaxf(M, pm), r = top == -INFINITY ? 0.f : top;
-            l = fmaf(l, ex2(M - r), pl * ex2(pm - r));
-            M = top;
-          }
-          const float sk = a.sinks ? a.sinks[done.h0 + m - row_in(m) * n_h] * LOG2E : -INFINITY, mm = fmaxf(warp_max(M), sk), r = mm == -INFINITY ? 0.f : mm;
-          l = warp_sum(l * ex2(M - r)) + (a.sinks ? ex2(sk - r) : 0.f);
-          if (lane == 0) {
-            sm_w[m] = r;
-            sm_w[16 + m] = l;
-          }
-        }
-        __syncthreads();
-        // four entries of a column to a thread, eight pieces in flight; with few columns the pieces go to several groups of threads
-        const int quads = live * (HDP / 4), groups = min(max(Q8_THREADS / quads, 1), n_pieces > 8 ? Q8_WARPS : 1);
-        for (int x0 = 0; x0 < quads * groups; x0 += Q8_THREADS) {
-          const int x = x0 + tid, part = x / quads, q = x - part * quads, m = q / (HDP / 4), i = q % (HDP / 4) * 4;
-          float v[4] = {0.f, 0.f, 0.f, 0.f};
-          if (part < groups) {
-            const float r = sm_w[m];
-            const int from = n_pieces * part / groups, to = n_pieces * (part + 1) / groups;
-            for (int b0 = from; b0 < to; b0 += 8) {
-              float pm[8];
-              float4 pv[8];
-#pragma unroll
-              for (int b = 0; b < 8; ++b) {
-                const float* p = piece(min(b0 + b, to - 1)) + m * (HDP + 4);
-                pm[b] = load_float(p + HDP);
-                asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(pv[b].x), "=f"(pv[b].y), "=f"(pv[b].z), "=f"(pv[b].w) : "l"(p + i) : "memory");
-              }
-#pragma unroll
-              for (int b = 0; b < 8; ++b)
-                if (b0 + b < to) {
-                  const float w = ex2(pm[b] - r);
-                  v[0] = fmaf(w, pv[b].x, v[0]);
-                  v[1] = fmaf(w, pv[b].y, v[1]);
-                  v[2] = fmaf(w, pv[b].z, v[2]);
-                  v[3] = fmaf(w, pv[b].w, v[3]);
-                }
-            }
-          }
-          if (groups > 1) {       // one round of threads then: the groups' sums are added in their order
-            float4* sum = reinterpret_cast<float4*>(sm_acc);
-            if (part > 0 && part < groups) sum[x - quads] = make_float4(v[0], v[1], v[2], v[3]);
-            __syncthreads();
-            if (part > 0) continue;
-            for (int k = 0; k < groups - 1; ++k) {
-              const float4 o4 = sum[k * quads + q];
-              v[0] += o4.x;
-              v[1] += o4.y;
-              v[2] += o4.z;
-              v[3] += o4.w;
-            }
-          }
-          if (part < groups) {
-            const float l = sm_w[16 + m];
-            const int h = done.h0 + m - row_in(m) * n_h;
-            TT* out = static_cast<TT*>(a.out) + (size_t)(done.it.row0 + row_in(m)) * a.out_ld + h * hd;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (dim_of(i + e) < hd) from_f32(out[dim_of(i + e)], l == 0.f ? 0.f : v[e] / l);
-          }
-        }
+        const unsigned drawn = atomicAdd(a.counters + (size_t)done.item * n_hg + done.hg, 1u);
+        if (more) ticket0 = drawn; else ticket1 = drawn;
       }
     }
     if (!more) break;
     __syncthreads();      // the next piece's queries and sums go where this one's were
+  }
+  if (!owed) return;
+
+  // The last one to finish a piece of an item merges them.  The cuts left inside the item: the piece behind cut c is block c's, the first
+  // piece that of the block before.
+  auto pieces_of = [&](int item, int hg, int& b_first) {
+    const long long begin = (long long)hg * total + before[item], end = begin + before[item + 1] - before[item];
+    b_first = quotient(begin + slack, per, per_inv);
+    return quotient(end - slack - 1, per, per_inv) - b_first + 1;
+  };
+  if (tid == Q8_THREADS - 32) {
+    bool last[2] = {false, false};
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+      if (owed >> w & 1) {
+        int b_first;
+        last[w] = (w ? ticket1 : ticket0) == (unsigned)(pieces_of(sm_i[4 + 2 * w], sm_i[5 + 2 * w], b_first) - 1);
+        sm_i[w] = last[w];
+      }
+    __threadfence();
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+      if (last[w]) a.counters[(size_t)sm_i[4 + 2 * w] * n_hg + sm_i[5 + 2 * w]] = 0;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int w = 0; w < 2; ++w) {
+    if (!(owed >> w & 1) || !sm_i[w]) continue;
+    const int item = sm_i[4 + 2 * w], hg = sm_i[5 + 2 * w], hk = a.head_blocks == 1 ? hg : hg / a.head_blocks, hb = hg - hk * a.head_blocks, h0 = hk * group + hb * a.heads_per;
+    const int n_h = min(a.heads_per, group - hb * a.heads_per), live = (a.cu_rows ? item_seq[item] : 1) * n_h, row0 = item_row[item];
+    const int n_h_inv = inverse(n_h);
+    auto row_in = [&](int m) { return m * n_h_inv >> 16; };
+    auto dim_of = [&](int i) { return ((i >> 1) & 7) * (HDP / 8) + (i >> 4) * 2 + (i & 1); };
+    int b_first;
+    const int n_pieces = pieces_of(item, hg, b_first);
+    auto piece = [&](int b) { return a.part + (size_t)(2 * (b_first + b) + (b == 0)) * NQ * (HDP + 4); };
+    // four entries of a column to a thread, eight pieces in flight; with few columns the pieces go to several groups of threads
+    const int quads = live * (HDP / 4), groups = n_pieces <= 8 || 2 * quads > Q8_THREADS ? 1 : (4 * quads > Q8_THREADS ? 2 : 4), shift = groups >> 1;      // (log2 of 1, 2, 4)
+    auto part_of = [&](int x) { return groups == 1 ? x >= quads : (x >= quads) + (x >= 2 * quads) + (groups > 2 ? (x >= 3 * quads) + (x >= 4 * quads) : 0); };
+    float pm[8];
+    float4 pv[8];
+    auto fetch = [&](int b0, int to, int m, int i) {
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        const float* p = piece(min(b0 + b, to - 1)) + m * (HDP + 4);
+        pm[b] = load_float(p + HDP);
+        asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(pv[b].x), "=f"(pv[b].y), "=f"(pv[b].z), "=f"(pv[b].w) : "l"(p + i) : "memory");
+      }
+    };
+    {      // the first of them beside the maxima and denominators
+      const int part = part_of(tid), q = tid - part * quads;
+      if (part < groups) fetch(n_pieces * part >> shift, n_pieces * (part + 1) >> shift, q / (HDP / 4), q % (HDP / 4) * 4);
+    }
+    // every column's maximum and denominator over the pieces
+    for (int m = warp; m < live; m += Q8_WARPS) {
+      float M = -INFINITY, l = 0.f;
+      for (int b = lane; b < n_pieces; b += 32) {
+        const float* p = piece(b) + m * (HDP + 4) + HDP;
+        const float pm = load_float(p), pl = load_float(p + 1), top = fmaxf(M, pm), r = top == -INFINITY ? 0.f : top;
+        l = fmaf(l, ex2(M - r), pl * ex2(pm - r));
+        M = top;
+      }
+      const float sk = a.sinks ? a.sinks[h0 + m - row_in(m) * n_h] * LOG2E : -INFINITY, mm = fmaxf(warp_max(M), sk), r = mm == -INFINITY ? 0.f : mm;
+      l = warp_sum(l * ex2(M - r)) + (a.sinks ? ex2(sk - r) : 0.f);
+      if (lane == 0) {
+        sm_w[m] = r;
+        sm_w[16 + m] = l;
+      }
+    }
+    __syncthreads();
+    for (int x0 = 0; x0 < quads * groups; x0 += Q8_THREADS) {
+      const int x = x0 + tid, part = part_of(x), q = x - part * quads, m = q / (HDP / 4), i = q % (HDP / 4) * 4;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (part < groups) {
+        const float r = sm_w[m];
+        const int from = n_pieces * part >> shift, to = n_pieces * (part + 1) >> shift;
+        for (int b0 = from; b0 < to; b0 += 8) {
+          if (x0 > 0 || b0 > from) fetch(b0, to, m, i);
+#pragma unroll
+          for (int b = 0; b < 8; ++b)
+            if (b0 + b < to) {
+              const float f = ex2(pm[b] - r);
+              v[0] = fmaf(f, pv[b].x, v[0]);
+              v[1] = fmaf(f, pv[b].y, v[1]);
+              v[2] = fmaf(f, pv[b].z, v[2]);
+              v[3] = fmaf(f, pv[b].w, v[3]);
+            }
+        }
+      }
+      if (groups > 1) {       // one round of threads then: the groups' sums are added in their order
+        float4* sum = reinterpret_cast<float4*>(sm_acc);
+        if (part > 0 && part < groups) sum[x - quads] = make_float4(v[0], v[1], v[2], v[3]);
+        __syncthreads();
+        if (part > 0) continue;
+        for (int k = 0; k < groups - 1; ++k) {
+          const float4 o4 = sum[k * quads + q];
+          v[0] += o4.x;
+          v[1] += o4.y;
+          v[2] += o4.z;
+          v[3] += o4.w;
+        }
+      }
+      if (part < groups) {
+        const float l = sm_w[16 + m];
+        const int h = h0 + m - row_in(m) * n_h;
+        TT* out = static_cast<TT*>(a.out) + (size_t)(row0 + row_in(m)) * a.out_ld + h * hd;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (dim_of(i + e) < hd) from_f32(out[dim_of(i + e)], l == 0.f ? 0.f : v[e] / l);
+      }
+    }
+    __syncthreads();      // (the second item's sums go where this one's were)
   }
 }
 
