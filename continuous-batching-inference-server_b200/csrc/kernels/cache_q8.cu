@@ -305,8 +305,8 @@ CBIS_EXPORT int cbis_kv_read_q8(const void* call) {
   int shift = 0;
   const int widest = vc && hd_v > hd ? hd_v : hd;
   while (shift < 5 && (vec ? N : 1) << shift < widest) ++shift;
-  // parts of a page: eight rows to a thread if there are blocks enough (23 requests of 90 to 1,100 tokens, 25 heads of 64: 28.2 us with
-  // four, 26.0 so), fewer rows for a few pages
+  // parts of a page: eight rows to a thread if there are blocks enough (23 requests of 90 to 1,100 tokens, 25 heads of 64: 8 % slower with
+  // four), fewer rows for a few pages
   const long long rows = (long long)heads * ps, per_block = 256 >> shift, pages = blocks * n_seg;
   long long parts = (rows + 8 * per_block - 1) / (8 * per_block), finest = (rows + per_block - 1) / per_block;
   if (pages * parts < 4 * 148) parts = (4 * 148 + pages - 1) / pages;

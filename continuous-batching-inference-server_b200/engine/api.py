@@ -51,7 +51,7 @@ class Engine:
         own position limit; for a model without one the default is what the pool is asked to hold (``num_pages`` or
         ``max_tokens``), else 32,768.  ``cache_dtype`` "int8" keeps keys and values in 8 bits, with a scale per token and head: about half
         the bytes per token of a bfloat16 cache, a quarter of a 32-bit one's.  Every query, a prompt's own too, sees the keys and
-        values as they are kept, so the logits do not depend on how a prompt is cut."""
+        values as they are kept, so how a prompt is cut changes the logits by rounding only."""
         if not torch.cuda.is_available():
             raise RuntimeError("the engine needs a CUDA device (sm_100a); there is no CPU path")
         self.model = load_model(model, dtype, device) if isinstance(model, str) else model

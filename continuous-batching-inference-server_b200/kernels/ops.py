@@ -917,21 +917,23 @@ def paged_prefill_q8(q, k_pages, v_pages, block_table, cu_rows, seg_start, seg_c
                  *(work or ()))
     if n_seg == 0 or n_rows == 0 or max_seg_rows <= 0:
         return
-    window, cap, keep = int(window), float(cap), int(keep)
+    window, cap, keep, max_context = int(window), float(cap), int(keep), int(max_context)
     if work is None or out.data_ptr() % 16 or out.stride(0) % 8 or not prefill_q8_reads_back(
             n_rows, max_seg_rows, n_seg, n_head, n_kv_head, head_dim, page_size, q.dtype, slopes, sinks, q_temp, rates, cap, keep):
         return _attention_q8(what, q, -1, -1, k_pages, v_pages, block_table, None, None, None, cu_rows, seg_start, seg0, n_seg,
                              int(max_seg_rows), out, scratch, counters, n_head, n_kv_head, head_dim, page_size, scale, window,
-                             int(max_context), slopes, sinks, q_temp, rates, cap, keep)
+                             max_context, slopes, sinks, q_temp, rates, cap, keep)
     far = 2 ** 30 + 1       # behind every position
-    window, keep, max_context = max(-far, min(window, far)), min(keep, far), min(int(max_context), far)
+    if not (-far <= window <= far and keep <= far and max_context <= far):
+        window, keep, max_context = max(-far, min(window, far)), min(keep, far), min(max_context, far)
     k, v = work
     tokens = min(max_context, abs(window) + max_seg_rows) if window else max_context
     blocks, wide = block_table.shape[1], q.dtype is _FLOAT32
     # (behind a window most parts would be empty)
     chunks = (1, 0) if window and not wide else _prefill_q8_chunks(max_seg_rows, n_seg, n_head, head_dim, max_context, q.dtype)
-    need = n_rows * n_head * chunks[0] * (head_dim + 4) if chunks[0] > 1 else 0
-    _q8_need(scratch.numel() >= need, what, f"scratch has {scratch.numel()} numbers and not {need}")
+    if chunks[0] > 1:
+        need = n_rows * n_head * chunks[0] * (head_dim + 4)
+        _q8_need(scratch.numel() >= need, what, f"scratch has {scratch.numel()} numbers and not {need}")
     _kv_read_q8(kc, ks, vc, vs, k, v, block_table.data_ptr() + 4 * seg0 * blocks, blocks, seg_start.data_ptr() + 4 * seg0,
                 seg_ctx.data_ptr() + 4 * seg0, n_seg, tokens, window, keep, 1 | (F32 if wide else BF16) << 1 | (not wide) << 2)
     args = (q, k, v, block_table, cu_rows, seg_start, out, seg0, n_seg, max_seg_rows, n_head, n_kv_head, head_dim, page_size, scale, window)
