@@ -821,6 +821,7 @@ def paged_decode_q8(qkv, k_off, v_off, k_pages, v_pages, block_table, row_seq, p
     ``q_temp``, ``rates``, ``cap``, ``keep``: as in ``paged_attention_generic``.  A row whose request is no row of the block table, or that sees no
     key, gets zeros; a page number that the cache does not have is passed over."""
     what = "paged_decode_q8"
+    _q8_need(v_pages is not None, what, "without values' pages: where one array stands for both, give the keys' pages twice")
     rows = qkv.shape[0]
     dtype_code(qkv.dtype)
     kc, ks = k_pages
@@ -889,6 +890,7 @@ def paged_prefill_q8(q, k_pages, v_pages, block_table, cu_rows, seg_start, seg_c
     attended to there (every page that a row sees is then one of the cache's).  Without ``work`` the first takes all.  The rest as in
     ``paged_decode_q8``."""
     what = "paged_prefill_q8"
+    _q8_need(v_pages is not None, what, "without values' pages: where one array stands for both, give the keys' pages twice")
     dtype_code(q.dtype)
     kc, ks = k_pages
     vc, vs = v_pages

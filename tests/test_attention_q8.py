@@ -520,3 +520,40 @@ def test_one_array_is_not_stored_twice():
     for v in (p, ops.Q8Pages(p.codes.view(p.codes.shape), p.scales)):
         with pytest.raises(ops.KernelError, match="of one array"):
             ops.paged_decode_q8(q, 128, 192, p, v, table, i, i, i, out, f, i, 4, 2, 32, 16, 1.0, 0, 32)
+
+
+def test_values_that_are_not_given_are_refused():
+    """Writing and reading back take None for one array of both; attention wants the values' pages named."""
+    from cbis_b200.kernels import ops
+    p = ops.q8_pages(2, 2, 16, 32, device="cpu")
+    q, out = torch.zeros(3, 256, dtype=BF), torch.zeros(3, 128, dtype=BF)
+    i, table, f = torch.zeros(4, dtype=torch.int32), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(1 << 16)
+    with pytest.raises(ops.KernelError, match="without values' pages"):
+        ops.paged_decode_q8(q, -1, -1, p, None, table, i, i, i, out, f, i, 4, 2, 32, 16, 1.0, 0, 32)
+    with pytest.raises(ops.KernelError, match="without values' pages"):
+        ops.paged_prefill_q8(q, p, None, table, i, i, i, i, out, 0, 2, 0, 3, 2, 4, 2, 32, 16, 1.0, 0, 32, f, i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("n", [1, 17, 33, 700])
+def test_the_only_key_of_a_tile_is_not_finite(ops, dtype, n):
+    """The newest key is the first of its tile, or the only one that the row sees: what a warp or block has of it is not-a-number with no
+    maximum, and the join has to keep that."""
+    for x in "kv":
+        c = make(ops, dtype, 4, 2, 64, 16, [n, 20], [1, 1], seed=n)
+        c[x].scales[int(c["table"][0, (n - 1) // 16]), 1, (n - 1) % 16] = math.nan
+        out = decode(ops, c).cpu().float().view(2, 4, 64)
+        assert torch.isnan(out[0, 2:]).all() and torch.isfinite(out[0, :2]).all() and torch.isfinite(out[1]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_the_first_key_of_a_long_chunk_is_not_finite(ops, hd):
+    """Row 0 sees this key alone, and behind a window of 50 later rows do not see it."""
+    for x in "kv":
+        c = make(ops, BF, 4, 2, hd, 16, [200], [200], seed=hd)
+        c[x].scales[int(c["table"][0, 0]), 1, 0] = math.nan
+        for window, seen in ((0, 200), (50, 50)):
+            out = prefill(ops, c, window, work=True).cpu().float().view(200, 4, hd)
+            assert torch.isfinite(out[:, :2]).all() and torch.isnan(out[:seen, 2:]).all() and torch.isfinite(out[seen:]).all()
