@@ -37,8 +37,10 @@
 // quotient would triple the load of the special-function units), else it goes through an exponential.
 //
 // CODED: keys and values are whole numbers (the codes of an 8-bit cache, exact in bfloat16) with a scale per key and one per value:
-// the scores are multiplied by the one and the weights, on their way to bfloat16, by the other, so nothing is rounded more often than
-// over keys and values in bfloat16.  The softmax threads bring a tile's 128 scales through the table's place in shared memory,
+// the scores are multiplied by the one and the weights by the other.  The weights then go to the tensor cores as two bfloat16 parts
+// (off by 2^-17; one part is off by 2^-8, which is as much again as the rounding of the result), as in the kernel that reads codes, so a
+// chunk's length does not choose its bits.  Shared memory has no room for two parts beside a second block: they go into tensor memory, over the scores that they
+// were made of, from where the product takes them as its first operand.  The softmax threads bring a tile's 128 scales through the table's place in shared memory,
 // asked for a tile ahead.  A value whose scale is not finite, or whose page the cache does not have, makes its key's scores not-a-number (its rows' results then are, and a row
 // that does not see it multiplies by zero).
 //
@@ -132,6 +134,11 @@ __device__ __forceinline__ void mma(unsigned tmem_d, unsigned long long da, unsi
   asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
                ::"r"(tmem_d), "l"(da), "l"(db), "r"(id), "r"(accumulate) : "memory");
 }
+// The same with A (rows in lanes, two values of a row to a column) in tensor memory.
+__device__ __forceinline__ void mma_from_tmem(unsigned tmem_d, unsigned tmem_a, unsigned long long db, unsigned id, unsigned accumulate) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+               ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(id), "r"(accumulate) : "memory");
+}
 __device__ __forceinline__ void commit(void* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s32(bar)) : "memory");
 }
@@ -183,6 +190,18 @@ __device__ __forceinline__ void tmem_st32(unsigned taddr, const float* v) {
         "r"(__float_as_uint(v[28])), "r"(__float_as_uint(v[29])), "r"(__float_as_uint(v[30])), "r"(__float_as_uint(v[31]))
       : "memory");
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// 32 columns of a row, not waited for.
+__device__ __forceinline__ void tmem_put32(unsigned taddr, const unsigned* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+        "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
+        "r"(v[30]), "r"(v[31])
+      : "memory");
 }
 
 // The largest of three; 2^x by ex2.approx.ftz, which flushes results below 2^-126 to zero: nothing beside a row's largest, which is at
@@ -426,13 +445,24 @@ paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         // O += P V: four steps of 16 keys; V is MN-major: 16 keys are two 1024-byte atoms, the other half of the
         // head dim KV_HALF_BYTES on
+        if constexpr (CODED) {      // the weights' two parts lie where their scores were, the small one behind the large one
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk) {
-          mma(tmem_o, dp + (unsigned)(((j % PBUF) * P_BYTES + kk * 32) >> 4), dv + (unsigned)((s * KV_BYTES + kk * 2048) >> 4), idesc(true, HD),
-              (j > 0 || kk > 0) ? 1u : 0u);
+          for (int part = 1; part >= 0; --part)
+#pragma unroll
+            for (int kk = 0; kk < BN / 16; ++kk)
+              mma_from_tmem(tmem_o, tmem_s + (j & 1) * BN + part * (BN / 2) + kk * 8, dv + (unsigned)((s * KV_BYTES + kk * 2048) >> 4),
+                            idesc(true, HD), (j > 0 || part == 0 || kk > 0) ? 1u : 0u);
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk) {
+            mma(tmem_o, dp + (unsigned)(((j % PBUF) * P_BYTES + kk * 32) >> 4), dv + (unsigned)((s * KV_BYTES + kk * 2048) >> 4), idesc(true, HD),
+                (j > 0 || kk > 0) ? 1u : 0u);
+          }
         }
         commit(&v_empty[s]);   // the values' stage is free again when these products have read it
         commit(&pv_done[j & 1]);
+        // CODED: the next scores go where these products read their weights, and products of other shapes are not bound to each other's order
+        if (CODED && j + 2 < n_tiles && !bar_wait(&pv_done[j & 1], (j >> 1) & 1)) { *abort_flag = 5; atomicExch(error, 16); break; }
         // the scores of tile j+2 go where those of tile j were: the softmax has read them (it said so with p_ready)
         if (j + 2 < n_tiles) ok = issue_qk(j + 2);
       }
@@ -574,7 +604,7 @@ paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       // P = exp2(S * scale - m) in bfloat16 into shared memory (rows of 64 keys, 128-byte swizzle), and its sum
       const unsigned long long scale2 = pack2(scale_log2e, scale_log2e), ref2 = pack2(-ref, -ref);
       unsigned long long psum = 0;
-      unsigned pk[8][4];
+      unsigned pk[8][4], pl[CODED ? 8 : 1][4];      // CODED: what the first part leaves over
 #pragma unroll
       for (int q8 = 0; q8 < 8; ++q8) {
         float4 vx[2];
@@ -596,14 +626,24 @@ paged_prefill_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           }
           __nv_bfloat162 b2 = __floats2bfloat162_rn(e0, e1);
           pk[q8][i] = *reinterpret_cast<unsigned*>(&b2);
+          if constexpr (CODED) {
+            b2 = __floats2bfloat162_rn(e0 - __uint_as_float(pk[q8][i] << 16), e1 - __uint_as_float(pk[q8][i] & 0xffff0000u));
+            pl[q8][i] = *reinterpret_cast<unsigned*>(&b2);
+          }
         }
       }
-      // the products that read this buffer of P last have done so by the time this tile's exponentials are there
-      if (j >= PBUF && !bar_wait(&pv_done[(j - PBUF) & 1], ((j - PBUF) >> 1) & 1)) { atomicExch(error, 16); ok = false; TC5_STOP }
-      unsigned char* prow = sP + (j % PBUF) * P_BYTES + r * 128;
+      if constexpr (CODED) {      // over this tile's scores, which every thread of the warp has read
+        tmem_put32(tmem_s + (j & 1) * BN + lane_addr, &pk[0][0]);
+        tmem_put32(tmem_s + (j & 1) * BN + BN / 2 + lane_addr, &pl[0][0]);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      } else {
+        // the products that read this buffer of P last have done so by the time this tile's exponentials are there
+        if (j >= PBUF && !bar_wait(&pv_done[(j - PBUF) & 1], ((j - PBUF) >> 1) & 1)) { atomicExch(error, 16); ok = false; TC5_STOP }
+        unsigned char* prow = sP + (j % PBUF) * P_BYTES + r * 128;
 #pragma unroll
-      for (int q8 = 0; q8 < 8; ++q8)
-        *reinterpret_cast<uint4*>(prow + ((q8 ^ (r & 7)) << 4)) = make_uint4(pk[q8][0], pk[q8][1], pk[q8][2], pk[q8][3]);   // swizzled
+        for (int q8 = 0; q8 < 8; ++q8)
+          *reinterpret_cast<uint4*>(prow + ((q8 ^ (r & 7)) << 4)) = make_uint4(pk[q8][0], pk[q8][1], pk[q8][2], pk[q8][3]);   // swizzled
+      }
       float psum0, psum1;
       unpack2(psum, psum0, psum1);
       l += psum0 + psum1;
