@@ -43,7 +43,7 @@ Q8Plan q8_plan(int n, int rows_of_seg, int n_head, int n_kv_head, int hd, int f3
       p.stages = x < 2 ? 3 : 2;
       p.join_cols = x % 2 == 0 ? 8 : least;
       if (p.join_cols > cols) p.join_cols = cols;
-      p.smem = q8_smem(stage, p.hdp + 8, ldq, p.stages, cols, p.join_cols, (int)p.items).bytes;
+      p.smem = q8_smem(stage, p.hdp + 8, ldq, p.stages, cols, p.join_cols, (int)p.items, q8_digits(f32 ? 3 : 2)).bytes;
       fits = fit_blocks * (p.smem + 1024) <= 228 * 1024;
     }
     if (fits || fit_blocks == 1) {

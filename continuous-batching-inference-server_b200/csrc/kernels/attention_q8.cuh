@@ -4,9 +4,10 @@
 //     s_j = scale ks_j (q . kc_j)  (a cap, a distance bias: as in the other attention kernels),   out = sum_j e^(s_j - m) vs_j vc_j / sum_j e^(s_j - m)
 // so the codes go through the tensor cores as they are and the scales meet the scores and the weights.  What bounds it is the codes'
 // bytes, read once: 2 (width + 4) per key and key/value head; close behind come the instructions, so few are spent on a code:
-//   * scores: mma.sync on signed bytes, keys as they lie in memory.  A query's numbers become whole numbers below 2^22 times a power of
-//     two of its own, cut into three signed bytes each, so the products are exact and a number is off by 2^-23 of the query's
-//     largest at most, for bfloat16 and for 32-bit rows alike;
+//   * scores: mma.sync on signed bytes, keys as they lie in memory.  A query's numbers become whole numbers times a power of two of its
+//     own, cut into signed bytes, so the products are exact: four bytes for bfloat16 rows and five for 32-bit rows, which hold a number
+//     to 2^-30 and 2^-38 of the query's LARGEST one.  So a channel keeps all its bits (8 and 24) down to 2^-22 and 2^-14 of the largest,
+//     and a large channel that no key has anything in costs the others nothing (three bytes left 2^-22: a channel 2^-10 of the largest kept 12 bits);
 //   * values: mma.sync on bfloat16, which holds a code exactly, with the weights times vs_j cut into two bfloat16 parts for bfloat16 rows
 //     (an error of 2^-17: one part costs 2^-9 of the result's size against 64 bits, as much as the rounding of the result itself) and
 //     into three for 32-bit rows.
@@ -198,6 +199,7 @@ struct Q8Place {
 
 // HDP: the width rounded up to 32, 64, 128 or 256; NT: columns of queries / 8; PARTS: bfloat16 parts of a weight (2: bfloat16 rows, 3:
 // 32-bit rows); EXT: kept first keys, a cap, a distance bias, a query temperature; FAST: the width is HDP and pages are a multiple of 16 keys.
+__host__ __device__ constexpr int q8_digits(int parts) { return parts + 2; }      // signed bytes of a query's number
 template <int HDP, int NT, int PARTS>
 struct Q8Shape {
   static constexpr int TPW = HDP >= 256 ? 1 : (HDP == 128 ? (NT == 1 ? 2 : 1) : 128 / HDP);        // tiles a warp takes through one update of its maxima and sums: a stage of its ring
@@ -214,13 +216,13 @@ struct Q8Shape {
 struct Q8Smem {
   int ring, join, stats, queries, columns, ints, items, bytes;
 };
-__host__ __device__ inline Q8Smem q8_smem(int stage, int lds, int ldq, int stages, int live, int jq, int n_items) {
+__host__ __device__ inline Q8Smem q8_smem(int stage, int lds, int ldq, int stages, int live, int jq, int n_items, int digits) {
   Q8Smem s;
   s.ring = 0;
   s.join = Q8_WARPS * stages * stage;
   s.stats = s.join + (Q8_WARPS * jq * lds * 4 > 2048 ? Q8_WARPS * jq * lds * 4 : 2048);      // (2 KB: the groups' sums of a merge)
   s.queries = s.stats + Q8_WARPS * 8 * 2 * 4;
-  s.columns = s.queries + 3 * live * ldq;
+  s.columns = s.queries + digits * live * ldq;
   s.ints = s.columns + 3 * 16 * 4;
   s.items = s.ints + 32;
   s.bytes = s.items + (4 * n_items + 1) * 4;
@@ -234,14 +236,15 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
   using TT = typename std::conditional<PARTS == 2, __nv_bfloat16, float>::type;
   constexpr int TPW = Shape::TPW, UNIT = Shape::UNIT, NQ = Shape::NQ, LDS = Shape::LDS, LDQ = Shape::LDQ, KS = HDP / 16;
   constexpr int STEPS = HDP / 32, VW = HDP / 32, PW = VW < 4 ? VW : 4;      // steps of the scores' product; words of a value that a lane takes, of one load
+  constexpr int DIGITS = q8_digits(PARTS);
   constexpr bool Q_IN_REGS = NT * HDP <= 128;
   extern __shared__ __align__(128) char smem[];
   const int cols = a.rows_per * a.heads_per;            // live columns at most
-  const Q8Smem at = q8_smem(Shape::STAGE, LDS, LDQ, a.stages, cols, a.join_cols, a.n_items);
+  const Q8Smem at = q8_smem(Shape::STAGE, LDS, LDQ, a.stages, cols, a.join_cols, a.n_items, DIGITS);
   float* sm_acc = reinterpret_cast<float*>(smem + at.join);          // [warp][join_cols][LDS]
   float* sm_m = reinterpret_cast<float*>(smem + at.stats);           // [warp][8]
   float* sm_l = sm_m + Q8_WARPS * 8;                                 // [warp][8]
-  int8_t* sm_q = reinterpret_cast<int8_t*>(smem + at.queries);       // [3][cols][LDQ] the queries' bytes, the highest first
+  int8_t* sm_q = reinterpret_cast<int8_t*>(smem + at.queries);       // [DIGITS][cols][LDQ] the queries' bytes, the highest first
   float* sm_f = reinterpret_cast<float*>(smem + at.columns);         // [16] a query's power of two, [16] maximum and [16] sum of merged pieces
   float* sm_w = sm_f + 16;
   int* sm_i = reinterpret_cast<int*>(smem + at.ints);                // [8]
@@ -472,7 +475,7 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
     const int live = cur.it.n_rows * cur.n_h, n_h = cur.n_h;
     const int n_h_inv = inverse(n_h);
     auto row_in = [&](int m) { return m * n_h_inv >> 16; };      // m / n_h, exact for m and n_h up to 16
-    // queries as three signed bytes a number, a warp to a query
+    // queries as signed bytes, a warp to a query
     for (int m = warp; m < live; m += Q8_WARPS) {
       float x[HDP / 32];
       unsigned top = 0;
@@ -488,12 +491,19 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
       const float f = __uint_as_float((unsigned)up << 23);
 #pragma unroll
       for (int i = 0; i < HDP / 32; ++i) {
-        const int v = top < 0x7f800000u ? __float2int_rn(x[i] * f) : 0;
-        const int lo = (int)(int8_t)v, v1 = (v - lo) >> 8, mid = (int)(int8_t)v1;
+        // the whole part, and what it leaves (exact, a half at most) as more bytes behind the point
+        const float y = x[i] * f;
+        int v = top < 0x7f800000u ? __float2int_rn(y) : 0, rest = top < 0x7f800000u ? __float2int_rn((y - (float)v) * (float)(1 << 8 * (DIGITS - 3))) : 0;
         int8_t* dst = sm_q + m * LDQ + (lane >> 2 & 3) * (HDP / 4) + i * 8 + (lane >> 4) * 4 + (lane & 3);      // number d = 32 i + 16 h + 4 t + byte: what lane t needs lies together
-        dst[0] = (int8_t)((v1 - mid) >> 8);
-        dst[cols * LDQ] = (int8_t)mid;
-        dst[2 * cols * LDQ] = (int8_t)lo;
+#pragma unroll
+        for (int digit = DIGITS - 1; digit > 0; --digit) {
+          if (digit == 2) v += rest;
+          int& from = digit > 2 ? rest : v;
+          const int low = (int)(int8_t)from;
+          dst[digit * cols * LDQ] = (int8_t)low;
+          from = (from - low) >> 8;
+        }
+        dst[0] = (int8_t)v;
       }
       if (lane == 0) sm_f[m] = top < 0x7f800000u ? __uint_as_float((unsigned)(254 - up) << 23) : __uint_as_float(0x7fc00000u);
     }
@@ -502,10 +512,10 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
     constexpr int QW = 2 * STEPS < 4 ? 2 * STEPS : 4;      // words of a load
     const unsigned q_at = (unsigned)__cvta_generic_to_shared(sm_q) + t * (HDP / 4);
     auto q_words = [&](int digit, int nt, int x, unsigned* w) { read_words<QW>(w, q_at + (digit * cols + min(nt * 8 + g, live - 1)) * LDQ + x * 8); };
-    unsigned qf[Q_IN_REGS ? 3 : 1][Q_IN_REGS ? NT : 1][Q_IN_REGS ? 2 * STEPS : 1];
+    unsigned qf[Q_IN_REGS ? DIGITS : 1][Q_IN_REGS ? NT : 1][Q_IN_REGS ? 2 * STEPS : 1];
     if constexpr (Q_IN_REGS) {
 #pragma unroll
-      for (int digit = 0; digit < 3; ++digit)
+      for (int digit = 0; digit < DIGITS; ++digit)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -579,33 +589,23 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
         hidden = hidden || fminf(kx[0], kx[1]) < 0.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          int sh[4], sd[4], sl[4];
+          int qk_sum[DIGITS][4];
 #pragma unroll
           for (int x0 = 0; x0 < STEPS; x0 += QW / 2) {
-            unsigned q0[QW], q1[QW], q2[QW];
-            if constexpr (Q_IN_REGS) {
 #pragma unroll
-              for (int w = 0; w < QW; ++w) {
-                q0[w] = qf[0][nt][2 * x0 + w];
-                q1[w] = qf[1][nt][2 * x0 + w];
-                q2[w] = qf[2][nt][2 * x0 + w];
-              }
-            } else {
-              q_words(0, nt, x0, q0);
-              q_words(1, nt, x0, q1);
-              q_words(2, nt, x0, q2);
-            }
+            for (int digit = 0; digit < DIGITS; ++digit) {
+              unsigned q[QW];
+              if constexpr (Q_IN_REGS) {
 #pragma unroll
-            for (int w = 0; w < QW; w += 2) {
-              const int x = x0 + w / 2;
-              if (x == 0) {
-                mma_16832_s8_first(sh, kw[x], q0[w], q0[w + 1]);
-                mma_16832_s8_first(sd, kw[x], q1[w], q1[w + 1]);
-                mma_16832_s8_first(sl, kw[x], q2[w], q2[w + 1]);
+                for (int w = 0; w < QW; ++w) q[w] = qf[digit][nt][2 * x0 + w];
               } else {
-                mma_16832_s8(sh, kw[x], q0[w], q0[w + 1]);
-                mma_16832_s8(sd, kw[x], q1[w], q1[w + 1]);
-                mma_16832_s8(sl, kw[x], q2[w], q2[w + 1]);
+                q_words(digit, nt, x0, q);
+              }
+#pragma unroll
+              for (int w = 0; w < QW; w += 2) {
+                const int x = x0 + w / 2;
+                if (x == 0) mma_16832_s8_first(qk_sum[digit], kw[x], q[w], q[w + 1]);
+                else mma_16832_s8(qk_sum[digit], kw[x], q[w], q[w + 1]);
               }
             }
           }
@@ -613,7 +613,10 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int c = e & 1;
-            float v = fmaf((float)sh[e], 65536.f, (float)(sd[e] * 256 + sl[e])) * (kx[e >> 1] * qx[nt][c]);
+            // two bytes' sums together hold in 32 bits (256 * 127 * 128 * 257 < 2^31)
+            const float low = (float)(qk_sum[DIGITS - 2][e] * 256 + qk_sum[DIGITS - 1][e]), high = (float)(qk_sum[DIGITS - 4][e] * 256 + qk_sum[DIGITS - 3][e]);
+            float v = DIGITS == 4 ? fmaf(low, 0x1p-8f, high * 256.f) : fmaf((float)qk_sum[0][e], 65536.f, fmaf(low, 0x1p-16f, high));
+            v *= kx[e >> 1] * qx[nt][c];
             if constexpr (EXT) {
               v = capped_score(v, a.cap);
               if (a.slopes) v -= distance_bias(qslope[nt][c], qrate[nt][c], (float)max(qp[nt][c] - (j0 + g + 8 * (e >> 1)), 0));

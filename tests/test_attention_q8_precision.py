@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import plain_q8
-from test_attention_q8 import BF, F32, decode, make, ops, prefill      # noqa: F401 (ops: a fixture)
+from test_attention_q8 import BF, F32, check, decode, make, ops, prefill      # noqa: F401 (ops: a fixture)
 
 
 def reference(c, window=0, rows=None):
@@ -65,3 +65,43 @@ def test_long_chunks(ops, H, G, hd, ps, window):      # noqa: F811
     for work in (True, False):
         out = prefill(ops, c, window, work=work).cpu().double()[list(rows)]
         assert norm(out - ref.to(BF).double()) / norm(ref) <= bound_16(ref, size), work
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("H,G,hd,ps", [(4, 4, 128, 16), (8, 2, 64, 16), (12, 1, 128, 16), (4, 1, 256, 16), (4, 4, 32, 16), (6, 3, 80, 5)])
+def test_decoding_rows_and_few_rows(ops, dtype, H, G, hd, ps):      # noqa: F811
+    c = make(ops, dtype, H, G, hd, ps, [17, 300, 700, 2000, 129, 64], [1] * 6, seed=hd)
+    ref, size = reference(c)
+    chunk = make(ops, dtype, H, G, hd, ps, [300, 700], [9, 30], seed=hd + 1)
+    chunk_ref, chunk_size = reference(chunk)
+    for out, ref, size in ((decode(ops, c), ref, size), (prefill(ops, chunk), chunk_ref, chunk_size)):
+        out = out.cpu().double()
+        if dtype == BF:
+            assert norm(out - ref.to(BF).double()) / norm(ref) <= bound_16(ref, size)
+        else:
+            assert norm(out - ref) / norm(ref) <= BOUND_32
+
+
+def with_a_large_channel(c, channel, large):
+    """One channel of the queries is far larger than the others, and no key has anything in it."""
+    c["q"].view(len(c["positions"]), c["H"], c["hd"])[:, :, channel] = large
+    c["k"].codes[..., channel] = 0
+    for k in c["held"][0]:
+        k[..., channel] = 0
+    return c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("H,G,hd,ps", [(4, 4, 64, 16), (4, 1, 128, 16), (2, 2, 32, 8), (12, 1, 64, 16), (2, 1, 256, 16), (2, 2, 48, 5)])
+@pytest.mark.parametrize("large,spread", [(3000.0, 1.0), (3000.0, 20.0), (-16000.0, 1.0)])
+def test_a_large_channel_costs_the_others_nothing(ops, dtype, H, G, hd, ps, large, spread):      # noqa: F811
+    """A dot product in 32 bits keeps every channel's own bits, and so the tolerance is the one of all other tests."""
+    c = with_a_large_channel(make(ops, dtype, H, G, hd, ps, [17, 300, 64], [1] * 3, seed=hd, spread=spread), 5, large)
+    check(c, decode(ops, c), hd ** -0.5)
+    c = with_a_large_channel(make(ops, dtype, H, G, hd, ps, [90, 200], [9, 20], seed=hd, spread=spread), hd - 1, large)
+    check(c, prefill(ops, c), hd ** -0.5)
+    if spread == 1.0 and dtype == F32:
+        ref, _ = reference(c)
+        assert norm(prefill(ops, c).cpu().double() - ref) / norm(ref) <= BOUND_32
