@@ -44,11 +44,15 @@ Q8Plan q8_plan(int n, int rows_of_seg, int n_head, int n_kv_head, int hd, int f3
       p.join_cols = x % 2 == 0 ? 8 : least;
       if (p.join_cols > cols) p.join_cols = cols;
       p.smem = q8_smem(stage, p.hdp + 8, ldq, p.stages, cols, p.join_cols, (int)p.items, q8_digits(f32 ? 3 : 2)).bytes;
-      fits = fit_blocks * (p.smem + 1024) <= 228 * 1024;
+      fits = p.smem <= Q8_MOST_SMEM && fit_blocks * (p.smem + 1024) <= 228 * 1024;      // (1 KB a block is the system's)
     }
-    if (fits || fit_blocks == 1) {
+    if (fits) {
       p.blocks = 148LL * fit_blocks;
       break;
+    }
+    if (fit_blocks == 1) {      // (not with Q8_MAX_ITEMS as it is)
+      p.items = Q8_MAX_ITEMS + 1;
+      return p;
     }
   }
   const long long pairs = p.items * n_kv_head * p.head_blocks, most = pairs * (max_context / (64 * tpw) + 2);      // no more blocks than there can be pieces

@@ -40,6 +40,7 @@
 namespace cbis {
 
 constexpr int Q8_WARPS = 4, Q8_THREADS = Q8_WARPS * 32, Q8_MAX_ITEMS = 4096;
+constexpr int Q8_MOST_SMEM = 227 * 1024;      // what a block may have: the launcher's plans and the kernels' limits go by it
 constexpr int Q8_PAIR = 6;      // what a pair costs beside its keys, in tiles
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -958,7 +959,7 @@ int q8_launch(const Q8Args& a, const Q8Plan& p, cudaStream_t st) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
   if (dev < 0 || dev >= 64 || !(set.load(std::memory_order_acquire) >> dev & 1)) {
-    e = allow_smem(kern, 200 * 1024);
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Q8_MOST_SMEM);
     if (e != cudaSuccess) return (int)e;
     if (dev >= 0 && dev < 64) set.fetch_or(1ull << dev, std::memory_order_release);
   }

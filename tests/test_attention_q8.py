@@ -557,3 +557,27 @@ def test_the_first_key_of_a_long_chunk_is_not_finite(ops, hd):
         for window, seen in ((0, 200), (50, 50)):
             out = prefill(ops, c, window, work=True).cpu().float().view(200, 4, hd)
             assert torch.isfinite(out[:, :2]).all() and torch.isnan(out[:seen, 2:]).all() and torch.isfinite(out[seen:]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("H,hd", [(8, 256), (16, 256), (16, 144), (8, 128), (4, 32)])
+def test_as_many_rows_as_a_call_takes(ops, dtype, H, hd):
+    """The rows' list lies in shared memory beside the tiles: with ``ATTENTION_Q8_MAX_ROWS`` of them the block is at its largest."""
+    n = ops.ATTENTION_Q8_MAX_ROWS
+    g = torch.Generator().manual_seed(hd)
+    c = make(ops, dtype, H, 1, hd, 16, [33, 1, 90, 200], [1] * 4, seed=H)
+    seq = torch.randint(0, 4, (n,), generator=g)
+    positions = (torch.rand(n, generator=g) * torch.tensor(c["ctx"])[seq]).to(torch.int32)
+    c.update(q=torch.randn(n, H * hd, generator=g).to(dtype), seq=seq.to(torch.int32), positions=positions)
+    check(c, decode(ops, c), hd ** -0.5, rows=[0, 1, n // 2, n - 2, n - 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_as_many_row_tiles_as_a_call_takes(ops, dtype):
+    """A chunk of one row a tile (16 query heads over one; in 32 bits at this width 8)."""
+    n, H = ops.ATTENTION_Q8_MAX_ROWS, 16 if dtype == BF else 8
+    c = make(ops, dtype, H, 1, 256, 64, [n], [n], seed=3)
+    assert ops.prefill_q8_takes(n, n, 1, H, 1, 256, 64, dtype)
+    check(c, prefill(ops, c), 1 / 16, rows=[0, 1, 2000, n - 1])
