@@ -798,9 +798,9 @@ attention_q8_kernel(const __grid_constant__ Q8Args a) {
             const int h = done.h0 + m - row_in(m) * n_h;
             float keep1 = 1.f;
             if (a.sinks) {
-              const float sk = a.sinks[h] * LOG2E, mm = fmaxf(M, sk);
-              keep1 = ex2(M - mm);
-              l = fmaf(l, keep1, ex2(sk - mm));
+              const float sk = a.sinks[h] * LOG2E, mm = fmaxf(M, sk), r = mm == -INFINITY ? 0.f : mm;      // (a head without a sink has -inf)
+              keep1 = ex2(M - r);
+              l = fmaf(l, keep1, ex2(sk - r));
             }
             if (d < hd) from_f32(static_cast<TT*>(a.out)[(size_t)(done.it.row0 + row_in(m)) * a.out_ld + h * hd + d], l == 0.f ? 0.f : v * keep1 / l);
           } else {

@@ -581,3 +581,23 @@ def test_as_many_row_tiles_as_a_call_takes(ops, dtype):
     c = make(ops, dtype, H, 1, 256, 64, [n], [n], seed=3)
     assert ops.prefill_q8_takes(n, n, 1, H, 1, 256, 64, dtype)
     check(c, prefill(ops, c), 1 / 16, rows=[0, 1, 2000, n - 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("H,G,hd,ps", [(4, 2, 64, 16), (3, 3, 32, 5), (12, 1, 128, 16)])
+def test_a_head_without_a_sink(ops, dtype, H, G, hd, ps):
+    """Its number is -inf: rows that see something get what they get without a sink, the others zeros, whether one block has the row's keys or
+    many (the third row's pages are all absent, the fourth row is of no request)."""
+    c = make(ops, dtype, H, G, hd, ps, [40, 3000, 3000, 1, 20], [1] * 5, seed=H)
+    c["table"][2], c["table"][4] = -1, -1
+    c["seq"][3] = -1
+    sinks = torch.tensor([-math.inf if h != 1 else 0.3 for h in range(H)])
+    out = decode(ops, c, sinks=sinks.cuda())
+    assert torch.all(out[2:] == 0)
+    check(c, out, hd ** -0.5, rows=[0, 1], sink=sinks.tolist())
+    c = make(ops, dtype, H, G, hd, ps, [90, 60], [7, 9], seed=H)
+    c["table"][1] = -1
+    out = prefill(ops, c, sinks=sinks.cuda())
+    assert torch.all(out[7:] == 0)
+    check(c, out, hd ** -0.5, rows=range(7), sink=sinks.tolist())
