@@ -95,7 +95,8 @@ __device__ __forceinline__ Q8Span q8_span(const Q8Args& a, const Q8Item& it) {
   const int last = it.pos0 + it.n_rows - 1, first_tile = first_seen(it.pos0, a.window) >> 4;
   s.nk = EXT ? min((kept_end(last, a.window, a.keep) + 15) >> 4, first_tile) : 0;
   s.skipped = first_tile - s.nk;
-  s.tiles = max(((min(last, a.max_blocks * a.ps - 1) >> 4) + 1) - s.skipped, 0);
+  const int held = (min(last, a.max_blocks * a.ps - 1) >> 4) + 1;      // behind the table's end a row sees the kept keys still
+  s.tiles = max(held - s.skipped, min(s.nk, held));
   return s;
 }
 

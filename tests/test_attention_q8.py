@@ -601,3 +601,28 @@ def test_a_head_without_a_sink(ops, dtype, H, G, hd, ps):
     out = prefill(ops, c, sinks=sinks.cuda())
     assert torch.all(out[7:] == 0)
     check(c, out, hd ** -0.5, rows=range(7), sink=sinks.tolist())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("H,G,hd,ps", [(4, 2, 64, 16), (3, 3, 48, 5)])
+def test_kept_keys_of_a_row_behind_the_table(ops, dtype, H, G, hd, ps):
+    """A position behind the block table's last block sees what it would if the table went on with pages that are not there: of the
+    window what lies in the table, and the kept first keys."""
+    c = make(ops, dtype, H, G, hd, ps, [160, 160, 160, 160], [1] * 4, seed=hd)
+    c["table"] = c["table"][:, :-(-160 // ps)].contiguous()
+    end, window, keep = 160, 40, 19
+    c["positions"] = torch.tensor([159, end + 20, end + 1000, 2 ** 31 - 1], dtype=torch.int32)
+    seen = [[*range(keep), *range(120, 160)], [*range(keep), *range(end + 20 - 39, end)], [*range(keep)], [*range(keep)]]
+    out = decode(ops, c, window, max_context=160, keep=keep).double().cpu()
+    start = c["positions"].clamp_max(2 ** 30).cuda()
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")      # noqa: E731
+    rows = torch.full_like(c["q"].cuda(), math.nan)
+    ops.paged_prefill_q8(c["q"].cuda(), c["k"], c["v"], c["table"].cuda(), i32(0, 1, 2, 3, 4), start, start + 1, start, rows, 0, 4, 0, 4, 1, H, G, hd, ps, hd ** -0.5,
+                         window, 160, *scratch(ops, 4, 1, 4, c), keep=keep)
+    for r, keys in enumerate(seen):
+        for h in range(H):
+            cols = slice(h * hd, (h + 1) * hd)
+            ref, weighted, size = plain_q8.attend(c["q"][r, cols].double(), c["held"][0][r][:, h // (H // G)], c["held"][1][r][:, h // (H // G)], 159, keys, hd ** -0.5)
+            tol = plain_q8.tolerance(dtype, ref, weighted, size, hd, len(keys))
+            assert ((out[r, cols] - ref).abs() <= tol).all() and ((rows[r, cols].double().cpu() - ref).abs() <= tol).all(), (r, h)
