@@ -668,8 +668,8 @@ def kv_read_q8(k_pages, v_pages, k_out, v_out, block_table, seg_start, seg_ctx, 
     ``v_out`` ``[pages, heads, page_size, width]``, for the tokens that the queries of request s (a row of ``block_table``) at
     positions ``seg_start[s]`` .. ``seg_ctx[s]`` - 1 see under ``window`` and ``keep`` (as in ``paged_attention_generic``); everything else in
     the two stays as it is.  ``max_tokens``: no request has more than so many such tokens, the kept first ones aside.
-    ``whole_pages``: what the request holds beside them in their pages is read back too; any kernel that takes pages then reads ``k_out`` and
-    ``v_out`` through the same block table.  ``v_pages`` None: one array."""
+    ``whole_pages``: what the request holds beside them in their pages is read back too; any kernel that takes pages then, and only then, reads
+    ``k_out`` and ``v_out`` through the same block table.  ``v_pages`` None: one array."""
     what = "kv_read_q8"
     kc, ks = k_pages
     vc, vs = (None, None) if v_pages is None or v_pages[0].data_ptr() == kc.data_ptr() else v_pages

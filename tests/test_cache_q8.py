@@ -174,3 +174,34 @@ def test_refusals():
 def test_the_plain_form_rounds_half_steps_to_even():
     c, s = plain_q8.quantise(torch.tensor([[254.0, 1.0, 3.0, -1.0, -5.0, 127.0]]))
     assert s.item() == 2.0 and c.tolist() == [[127.0, 0.0, 2.0, 0.0, -2.0, 64.0]]
+
+
+@pytest.mark.gpu
+def test_pages_read_back_are_there_for_the_kernel_behind(ops):
+    """The decode kernel asks for its first keys before it waits for the kernel ahead: read back and attended to one right after the other,
+    over pages that hold other numbers each time, the results are those of a stop in between."""
+    g = torch.Generator().manual_seed(2)
+    H, hd, ps, S, blocks = 8, 128, 16, 4, 24
+    pages = S * blocks
+    kp, vp = ops.q8_pages(pages, H, ps, hd), ops.q8_pages(pages, H, ps, hd)
+    ko, vo = (torch.zeros(pages, H, ps, hd, dtype=torch.bfloat16, device="cuda") for _ in "kv")
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")      # noqa: E731
+    table = torch.randperm(pages, generator=g).view(S, blocks).to(torch.int32).cuda()
+    ctx, seq, none = i32([384, 37, 200, 1]), i32([0, 1, 2, 3]), i32([-1] * 4)
+    q = torch.randn(S, H * hd, generator=g).to(torch.bfloat16).cuda()
+    for turn in range(20):
+        for p in (kp, vp):
+            p.codes.random_(-127, 128)
+            p.scales.uniform_(0.01, 0.03)
+        outs = []
+        for stop in (False, True):
+            out = torch.empty(S, H * hd, dtype=torch.bfloat16, device="cuda")
+            ko.fill_(turn)
+            vo.fill_(turn)
+            torch.cuda.synchronize()
+            ops.kv_read_q8(kp, vp, ko, vo, table, ctx - 1, ctx, 384, whole_pages=True)
+            if stop:
+                torch.cuda.synchronize()
+            ops.paged_decode_bf16(q, -1, -1, ko, vo, table, seq, ctx - 1, none, out, None, None, H, H, hd, ps, hd ** -0.5, 0, 1)
+            outs.append(out)
+        assert torch.equal(*outs)
