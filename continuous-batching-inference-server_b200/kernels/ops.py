@@ -679,7 +679,8 @@ def kv_read_q8(k_pages, v_pages, k_out, v_out, block_table, seg_start, seg_ctx, 
     if not (vc is not None and v_out is not None and len(shape) == 4 and kc.dtype is _INT8 and vc.dtype is _INT8 and ks.dtype is _FLOAT32
             and vs.dtype is _FLOAT32 and vc.shape[:3] == shape[:3] and len(vc.shape) == 4 and ks.shape == shape[:3] and vs.shape == shape[:3]
             and k_out.shape == shape and v_out.shape == vc.shape and v_out.dtype is k_out.dtype and kc.is_contiguous() and vc.is_contiguous()
-            and ks.is_contiguous() and vs.is_contiguous() and k_out.is_contiguous() and v_out.is_contiguous() and block_table.dtype is _INT32
+            and ks.is_contiguous() and vs.is_contiguous() and k_out.is_contiguous() and v_out.is_contiguous() and k_out.data_ptr() != v_out.data_ptr()
+            and block_table.dtype is _INT32
             and block_table.dim() == 2 and block_table.is_contiguous() and block_table.shape[1] > 0 and seg_start.dtype is _INT32 and seg_ctx.dtype is _INT32
             and seg_start.is_contiguous() and seg_ctx.is_contiguous() and seg_start.numel() >= S and seg_ctx.numel() >= S and keep >= 0
             and 0 <= dev == ks.get_device() == vc.get_device() == vs.get_device() == k_out.get_device() == v_out.get_device()
@@ -694,6 +695,7 @@ def kv_read_q8(k_pages, v_pages, k_out, v_out, block_table, seg_start, seg_ctx, 
         for o, c in outs:
             _q8_need(o is not None and o.dtype == k_out.dtype and o.shape == c.shape and c.shape[0] == shape[0] and o.is_contiguous(), what,
                      "the values' pages must be contiguous, of one type and of the codes' shape")
+        _q8_need(vc is None or k_out.numel() == 0 or k_out.data_ptr() != v_out.data_ptr(), what, "keys and values cannot be read back into the same pages")
         _q8_int32(what, "seg_start", seg_start, S)
         _q8_int32(what, "seg_ctx", seg_ctx, S)
         _q8_need(keep >= 0, what, "keep is negative")
@@ -902,7 +904,7 @@ def paged_prefill_q8(q, k_pages, v_pages, block_table, cu_rows, seg_start, seg_c
             and positions.numel() >= row0 + n_rows
             and q.get_device() == cu_rows.get_device() == seg_start.get_device() == seg_ctx.get_device() == positions.get_device()
             and (work is None or (work[0].dtype is q.dtype and work[1].dtype is q.dtype and work[0].shape == kc.shape and work[1].shape == vc.shape
-                                  and work[0].is_contiguous() and work[1].is_contiguous()
+                                  and work[0].is_contiguous() and work[1].is_contiguous() and work[0].data_ptr() != work[1].data_ptr()
                                   and q.get_device() == work[0].get_device() == work[1].get_device()))):
         _q8_attention_checks(what, q, k_pages, v_pages, block_table, out, scratch, counters, n_head, n_kv_head, head_dim, page_size, slopes,
                              sinks, rates, keep)
@@ -915,6 +917,8 @@ def paged_prefill_q8(q, k_pages, v_pages, block_table, cu_rows, seg_start, seg_c
         if work is not None:
             for o, p in zip(work, (k_pages, v_pages)):
                 _q8_need(o.dtype == q.dtype and o.shape == p.codes.shape and o.is_contiguous(), what, "work must be contiguous, of q's type and the codes' shape")
+            _q8_need(kc.data_ptr() == vc.data_ptr() or work[0].numel() == 0 or work[0].data_ptr() != work[1].data_ptr(), what,
+                     "work must be two arrays: keys and values cannot be read back into the same pages")
         _q8_here(what, q, kc, ks, vc, vs, block_table, cu_rows, seg_start, seg_ctx, positions, out, scratch, counters, slopes, sinks, rates,
                  *(work or ()))
     if n_seg == 0 or n_rows == 0 or max_seg_rows <= 0:

@@ -626,3 +626,18 @@ def test_kept_keys_of_a_row_behind_the_table(ops, dtype, H, G, hd, ps):
             ref, weighted, size = plain_q8.attend(c["q"][r, cols].double(), c["held"][0][r][:, h // (H // G)], c["held"][1][r][:, h // (H // G)], 159, keys, hd ** -0.5)
             tol = plain_q8.tolerance(dtype, ref, weighted, size, hd, len(keys))
             assert ((out[r, cols] - ref).abs() <= tol).all() and ((rows[r, cols].double().cpu() - ref).abs() <= tol).all(), (r, h)
+
+
+def test_keys_and_values_are_not_read_back_into_the_same_pages():
+    from cbis_b200.kernels import ops
+    kp, vp = ops.q8_pages(2, 2, 16, 32, device="cpu"), ops.q8_pages(2, 2, 16, 32, device="cpu")
+    q, out, w = torch.zeros(3, 256, dtype=BF), torch.zeros(3, 128, dtype=BF), torch.zeros(2, 2, 16, 32, dtype=BF)
+    i, table, f = torch.zeros(4, dtype=torch.int32), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(1 << 16)
+    with pytest.raises(ops.KernelError, match="the same pages"):
+        ops.kv_read_q8(kp, vp, w, w, table, i, i, 32)
+    call = lambda v, work: ops.paged_prefill_q8(q, kp, v, table, i, i, i, i, out, 0, 2, 0, 3, 2, 4, 2, 32, 16, 1.0, 0, 32, f, i, work)      # noqa: E731
+    with pytest.raises(ops.KernelError, match="the same pages"):
+        call(vp, (w, w))
+    for v, work in ((kp, (w, w)), (vp, (w, w.clone()))):      # one array for both may go to one place
+        with pytest.raises(ops.KernelError, match="no CPU path"):
+            call(v, work)
