@@ -52,3 +52,12 @@ def tolerance(dtype, ref, weighted, size, width, n_keys):
     moved = 2 * (width + 8) * 2.0 ** -23 * size + (n_keys + 64) * 2.0 ** -23
     half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -23
     return weighted * (moved + half) + ref.abs() * half + 1e-30
+
+
+def gpt_attention(h, c_attn_w, c_attn_b, c_proj_w, c_proj_b, n_head):
+    """``plain_gpt.attention`` with keys and values as an 8-bit cache holds them."""
+    T, d = h.shape
+    q, k, v = (x.reshape(T, n_head, d // n_head) for x in (h @ c_attn_w + c_attn_b).split(d, dim=1))
+    k, v = (codes * scale.double()[..., None] for codes, scale in (quantise(k), quantise(v)))
+    out = [attend(q[p, i], k[:, i], v[:, i], p, list(range(p + 1)), (d // n_head) ** -0.5)[0] for p in range(T) for i in range(n_head)]
+    return torch.stack(out).reshape(T, d) @ c_proj_w + c_proj_b
