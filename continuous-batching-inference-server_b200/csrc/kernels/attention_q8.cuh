@@ -2,8 +2,9 @@
 //
 // For the query q at position p over the keys j that it sees (codes kc_j, vc_j with scales ks_j, vs_j):
 //     s_j = scale ks_j (q . kc_j)  (a cap, a distance bias: as in the other attention kernels),   out = sum_j e^(s_j - m) vs_j vc_j / sum_j e^(s_j - m)
-// so the codes go through the tensor cores as they are and the scales meet the scores and the weights.  What bounds it is the codes'
-// bytes, read once: 2 (width + 4) per key and key/value head; close behind come the instructions, so few are spent on a code:
+// so the codes go through the tensor cores as they are and the scales meet the scores and the weights.  It cannot do without the codes'
+// bytes, read once: 2 (width + 4) per key and key/value head.  What bounds it now is the latency of dependent instructions, three warps a
+// scheduler, and the joins at the ends of pieces (neither memory nor a pipe is full), so few instructions are spent on a code:
 //   * scores: mma.sync on signed bytes, keys as they lie in memory.  A query's numbers become whole numbers times a power of two of its
 //     own, cut into signed bytes, so the products are exact: four bytes for bfloat16 rows and five for 32-bit rows, which hold a number
 //     to 2^-30 and 2^-38 of the query's LARGEST one.  So a channel keeps all its bits (8 and 24) down to 2^-22 and 2^-14 of the largest,
@@ -24,12 +25,13 @@
 // evenly over the blocks: every block works out its part from the positions on the device.  A cut that would leave a short end of a
 // pair is moved to the pair's end: a pair that lies in several blocks is merged by the last one to finish it.
 //
-// Measured on one B200, in a graph (copies run at 6.45 TB/s): 64 rows of 120 to 1,400 keys under 16 heads of 128 50.6 us, 4.1 TB/s; 5 rows
+// Measured on one B200, in a graph (copies run at 6.45 TB/s): 64 rows of 120 to 1,400 keys under 16 heads of 128 52.1 us, 4.0 TB/s; 5 rows
 // of 7,000 to 30,011 keys, 16 heads over 4, 29.4 us, 3.1 TB/s (over a bfloat16 cache 59 and 71 us); one row of 1,100 keys, 16 heads,
-// 10.0 us, of which 2 go by before the first keys are asked for, 1.5 until they are there and 4 in the join, the ticket and the merge;
-// in 32 bits 16 rows of 300 to 2,000 keys, 8 heads of 32, 13.4 us; chunks of 2 to 7 rows of twelve requests, 25 heads of 64, 17.1 us.
-// A tile of a head takes some 450 warp instructions, 128 of them to make bfloat16 numbers of the values' codes; the schedulers are
-// busy 44 % of the time, with three warps each.
+// 10.0 us, of which 2 go by before the first keys are asked for, 1.5 until they are there and 4 in the join, the ticket and the merge
+// (where the kernel stores the current token, which takes a fence and a barrier before a piece's first keys are asked for, 56.1, 30.7 and 11.0); in 32 bits 16 rows of
+// 300 to 2,000 keys, 8 heads of 32, 13.6 us; chunks of 2 to 7 rows of twelve requests, 25 heads of 64, 17.4 us.
+// A tile of a head takes some 475 warp instructions, 128 of them to make bfloat16 numbers of the values' codes; the schedulers are
+// busy 46 % of the time, with three warps each.
 #pragma once
 #include "cache_q8.cuh"
 #include "mma_sync.cuh"

@@ -3,7 +3,7 @@
 //
 // Both are bound by their bytes once there are some megabytes of them, and by the launch below that.  One B200, in a graph: 8 tokens of 16
 // heads of 128 written in 1.6 us, 2,048 in 9.9 (25.4 MB read and written); 23 requests of 90 to 1,100 tokens, 25 heads of 64, read back in
-// 29.5 us (134.9 MB, 4.6 TB/s), 32,767 tokens of 8 heads of 32 to 32 bits in 14.4 (86 MB, some of it from L2).
+// 29.4 us (134.9 MB, 4.6 TB/s), 32,767 tokens of 8 heads of 32 to 32 bits in 14.8 (86 MB, some of it from L2).
 #include "cache_q8.cuh"
 #include "packed.cuh"
 #include <string.h>

@@ -860,11 +860,11 @@ def prefill_q8_reads_back(n_rows: int, max_seg_rows: int, n_seg: int, n_head: in
 
     In bfloat16 that is the tcgen05 kernel over codes as they are.  For every thousand keys it takes some 0.12 us a tile of 128 rows and head
     (0.08 at head size 64), however few of the rows there are, and reading back 0.0011 us a number of a token; the kernel that
-    reads codes takes 0.004 us a row and head of 128.  16 heads of 128 behind 2,000 keys: 32 rows 25.1 us here and 29.5 there, 64 rows
-    32.7 and 29.9, 128 rows 41.7 and 31.3, 512 rows behind 8,192 294 and 102; twelve requests of 16 rows behind 1,000 keys 45.2 and 69.0,
-    over 4 key/value heads 45.2 and 47.6, of 32 heads over 4 of 64 41.7 and 64.8.  In 32 bits the kernel that reads codes multiplies on the
-    tensor cores and is the faster one: 512 rows of 8 heads of 32 behind 8,192 85 us and 131, 256 rows of 16 heads over 4 of 64 behind 2,000
-    43 and 75."""
+    reads codes takes 0.004 us a row and head of 128.  16 heads of 128 behind 2,000 keys: 32 rows 25.0 us here and 28.9 there, 64 rows
+    32.1 and 30.0, 128 rows 41.8 and 31.2, 512 rows behind 8,192 304 and 101; twelve requests of 16 rows behind 1,000 keys 43.4 and 69.3,
+    over 4 key/value heads 43.5 and 46.7, of 32 heads over 4 of 64 41.4 and 63.6.  In 32 bits the kernel that reads codes multiplies on the
+    tensor cores and is the faster one: 512 rows of 8 heads of 32 behind 8,192 92 us and 132, 256 rows of 16 heads over 4 of 64 behind 2,000
+    47 and 83."""
     wide = dtype == torch.float32
     if page_size & (page_size - 1) or slopes is not None or q_temp is not None or (
             head_dim > 128 or sinks is not None or cap or keep if wide else head_dim not in (64, 128) or not 8 <= page_size <= 128 or not USE_TCGEN05):
